@@ -509,4 +509,7 @@ int sl8_read_device_status(void* workspace, void* stream);
 #ifdef __cplusplus
 }
 #endif
+
+#include "superl8_b200_paged.h" /* rotary positions and the paged int8 K/V cache */
+
 #endif /* SUPERL8_B200_H_ */

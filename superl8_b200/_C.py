@@ -524,3 +524,217 @@ def attn_bwd(q, k, v, o, do_, lse, scale, causal=False, *, backend=_lib.SL8_BACK
         _bwd_ws[(q.device.index, torch.cuda.current_stream(q.device).cuda_stream)] = ws
     _lib.check(rc, "attn_bwd", 3 if (M and N and q.numel() and k.numel()) else 0)
     return dq, dk, dv
+
+
+# ---- rotary positions and the paged int8 K/V cache (include/superl8_b200_paged.h) ----
+# The compiled twin is csrc/torch_ext/sl8_torch_paged.cpp: the same checks in the same words.
+
+
+def _rows(t, aligned):
+    """``t`` itself when the kernels can take its rows in place, else a contiguous copy."""
+    ok = t.stride(3) == 1 or t.shape[3] == 1
+    if aligned and ok:
+        ok = t.data_ptr() % 16 == 0 and all(t.shape[d] <= 1 or t.stride(d) % 8 == 0 for d in range(3))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _steps(t, name):
+    return {f"{name}_stride_{c}": 0 if t.shape[d] == 1 else t.stride(d) for d, c in enumerate("bhs")}
+
+
+def _on(t, like, what):
+    _check(t.is_cuda, f"{what}: all inputs must be CUDA tensors")
+    _check(t.device == like.device, f"{what}: all inputs must be on the same device")
+
+
+def _rope_args(positions, inv_freq, freq_axis, like, B, S, D, what):
+    """The fields that RopeParams and AppendParams share, and the rotated width."""
+    _on(inv_freq, like, what)
+    _check(inv_freq.dtype == torch.float32 and inv_freq.dim() == 1 and inv_freq.is_contiguous(),
+           f"{what}: inv_freq must be a contiguous float32 [rot / 2] tensor")
+    _check(2 * inv_freq.numel() <= D, f"{what}: 2 * len(inv_freq) must not exceed the head dim")
+    f = dict(inv_freq=inv_freq.data_ptr(), rot=2 * inv_freq.numel(), n_axes=1)
+    if positions is not None:
+        p = positions
+        shapes = f"{what}: positions must be [S], [B, S] or [axes, B, S]"
+        _on(p, like, what)
+        _check(p.dtype in (torch.int32, torch.int64), f"{what}: positions must be int32 or int64")
+        _check(1 <= p.dim() <= 3, shapes)
+        _check(p.shape[-1] == S and (p.dim() < 2 or p.shape[-2] in (B, 1)) and (p.dim() < 3 or 1 <= p.shape[0] <= 255), shapes)
+        f.update(positions=p.data_ptr(), pos_is_64=int(p.dtype == torch.int64), pos_stride_s=p.stride(-1),
+                 pos_stride_b=p.stride(-2) if p.dim() >= 2 and p.shape[-2] != 1 else 0,
+                 pos_stride_axis=p.stride(0) if p.dim() == 3 else 0, n_axes=p.shape[0] if p.dim() == 3 else 1)
+    if freq_axis is not None:
+        _on(freq_axis, like, what)
+        _check(freq_axis.dtype == torch.uint8 and freq_axis.dim() == 1 and freq_axis.is_contiguous()
+               and freq_axis.numel() == inv_freq.numel(), f"{what}: freq_axis must be a contiguous uint8 [rot / 2] tensor")
+        f.update(freq_axis=freq_axis.data_ptr())
+    _check(f["n_axes"] == 1 or freq_axis is not None, f"{what}: positions with several axes need freq_axis")
+    return f
+
+
+def rope(q, k, positions, inv_freq, freq_axis=None, interleaved=False, inverse=False):
+    """Rotary positions on q and (optionally) k [B, H, S, D]: (q_out, k_out or None).  ``inverse``
+    turns by the opposite angle (the gradient)."""
+    what = "superl8_b200 apply_rope"
+    if _compiled():
+        r = _ext.rope(q, k, positions, inv_freq, freq_axis, bool(interleaved), bool(inverse))
+        _lib.launches += 1 if (r[0].numel() or (k is not None and k.numel())) else 0
+        return r
+    _check(q.is_cuda, f"{what}: all inputs must be CUDA tensors")
+    _check(q.dim() == 4, f"{what}: expect [B,H,S,D]")
+    _check(q.dtype in _DTYPE, f"{what}: q must be float16, bfloat16 or float32")
+    B, Hq, S, D = q.shape
+    _check(D % 2 == 0 and D > 0, f"{what}: the head dim must be even")
+    q = _rows(q, False)
+    q_out = torch.empty_like(q)
+    f = dict(q=q.data_ptr(), q_out=q_out.data_ptr(), **_steps(q, "q"), **_steps(q_out, "q_out"), B=B, Hq=Hq, S=S, D=D)
+    k_out = None
+    if k is not None:
+        _on(k, q, what)
+        _check(k.dim() == 4 and k.shape[0] == B and k.shape[2] == S and k.shape[3] == D,
+               f"{what}: q and k must agree in batch, length and head dim")
+        _check(k.dtype == q.dtype, f"{what}: q and k must share one dtype")
+        k = _rows(k, False)
+        k_out = torch.empty_like(k)
+        f.update(k=k.data_ptr(), k_out=k_out.data_ptr(), Hkv=k.shape[1], **_steps(k, "k"), **_steps(k_out, "k_out"))
+    f.update(_rope_args(positions, inv_freq, freq_axis, q, B, S, D, what))
+    if q.numel() or (k is not None and k.numel()):
+        p = _lib.RopeParams(dtype=_DTYPE[q.dtype], interleaved=int(bool(interleaved)), inverse=int(bool(inverse)), **f)
+        with torch.cuda.device(q.device):
+            rc = _lib.load().sl8_rope(C.byref(p), _stream(q.device))
+        _lib.check(rc, "apply_rope", 1)
+    return q_out, k_out
+
+
+def _paged_cache(k_i8, k_scale, v_i8, v_scale, table, lens, what):
+    _check(k_i8.is_cuda, f"{what}: all inputs must be CUDA tensors")
+    for t in (k_scale, v_i8, v_scale, table, lens):
+        _on(t, k_i8, what)
+    _check(k_i8.dtype == torch.int8 and v_i8.dtype == torch.int8, f"{what}: the cache's codes must be int8")
+    _check(k_i8.dim() == 4 and k_i8.shape == v_i8.shape and k_i8.is_contiguous() and v_i8.is_contiguous(),
+           f"{what}: the cache's codes must be contiguous [pages, H_kv, page_size, D], K like V")
+    _check(k_scale.dtype == torch.float32 and v_scale.dtype == torch.float32, f"{what}: scales must be float32")
+    _check(k_scale.dim() == 2 and k_scale.shape == k_i8.shape[:2] and k_scale.shape == v_scale.shape
+           and k_scale.is_contiguous() and v_scale.is_contiguous(), f"{what}: scales must be contiguous [pages, H_kv]")
+    pages, Hkv, page, D = k_i8.shape
+    _check(page in (16, 32, 64, 128, 256), f"{what}: page size must be 16/32/64/128/256, got {page}")
+    _check(D in (32, 64, 128, 256), f"{what}: head dim must be 32/64/128/256, got {D}")
+    _check(table.dtype == torch.int32 and table.dim() == 2 and (table.shape[1] <= 1 or table.stride(1) == 1),
+           f"{what}: block_table must be int32 [B, pages per sequence] with contiguous rows")
+    _check(lens.dtype == torch.int32 and lens.dim() == 1 and lens.is_contiguous() and lens.shape[0] == table.shape[0],
+           f"{what}: context_lens must be a contiguous int32 [B] tensor")
+    return _lib.PagedCache(k=k_i8.data_ptr(), v=v_i8.data_ptr(), k_scale=k_scale.data_ptr(), v_scale=v_scale.data_ptr(),
+                           block_table=table.data_ptr(), table_stride=table.stride(0), context_lens=lens.data_ptr(),
+                           num_pages=pages, Hkv=Hkv, page_size=page, D=D, max_pages=table.shape[1])
+
+
+def _lens_ptr(t, like, B, name, what):
+    if t is None:
+        return None
+    _on(t, like, what)
+    _check(t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous() and t.shape[0] == B,
+           f"{what}: {name} must be a contiguous int32 [B] tensor")
+    return t.data_ptr()
+
+
+def kv_append_paged(k, v, k_i8, k_scale, v_i8, v_scale, block_table, context_lens, new_lens=None, q=None, positions=None,
+                    inv_freq=None, freq_axis=None, interleaved=False):
+    """Stores new keys and values [B, H_kv, M, D] in the pages of an int8 cache (rotated on the way when
+    ``inv_freq`` is given); returns the rotated q, or None without one."""
+    what = "superl8_b200 kv_append_paged"
+    if _compiled():
+        r = _ext.kv_append_paged(k, v, k_i8, k_scale, v_i8, v_scale, block_table, context_lens, new_lens, q, positions,
+                                 inv_freq, freq_axis, bool(interleaved))
+        _lib.launches += 1 if (k.numel() or (q is not None and q.numel())) else 0
+        return r
+    cache = _paged_cache(k_i8, k_scale, v_i8, v_scale, block_table, context_lens, what)
+    _on(k, k_i8, what)
+    _on(v, k_i8, what)
+    _check(k.dtype in (torch.float16, torch.bfloat16), f"{what}: k must be float16 or bfloat16")
+    _check(v.dtype == k.dtype, f"{what}: k and v must share one dtype")
+    _check(k.dim() == 4 and k.shape == v.shape, f"{what}: expect k and v [B,H,S,D] of one shape")
+    B, Hkv, M, D = k.shape
+    _check(B == context_lens.shape[0] and Hkv == cache.Hkv and D == cache.D,
+           f"{what}: k and v must match the cache and block_table in batch, heads and head dim")
+    f = dict(new_lens=_lens_ptr(new_lens, k_i8, B, "new_lens", what), n_axes=1)
+    _check(inv_freq is not None or (q is None and positions is None and freq_axis is None),
+           f"{what}: q, positions and freq_axis need inv_freq")
+    if inv_freq is not None:
+        f.update(_rope_args(positions, inv_freq, freq_axis, k_i8, B, M, D, what))
+        _check(f["rot"] % 16 == 0, f"{what}: 2 * len(inv_freq) must be a multiple of 16")
+    k, v = _rows(k, True), _rows(v, True)
+    f.update(k_new=k.data_ptr(), v_new=v.data_ptr(), **_steps(k, "k"), **_steps(v, "v"))
+    q_out = None
+    if q is not None:
+        _on(q, k_i8, what)
+        _check(q.dtype == k.dtype, f"{what}: q must have the dtype of k and v")
+        _check(q.dim() == 4 and q.shape[0] == B and q.shape[2] == M and q.shape[3] == D,
+               f"{what}: q must be [B,H_q,S,D] with the batch, length and head dim of k")
+        q = _rows(q, True)
+        q_out = torch.empty_like(q)
+        f.update(q=q.data_ptr(), q_out=q_out.data_ptr(), Hq=q.shape[1], **_steps(q, "q"), **_steps(q_out, "q_out"))
+    if k.numel() or (q is not None and q.numel()):
+        p = _lib.AppendParams(B=B, M=M, dtype=_DTYPE[k.dtype], interleaved=int(bool(interleaved)), **f)
+        with torch.cuda.device(k_i8.device):
+            rc = _lib.load().sl8_kv_append_paged(C.byref(cache), C.byref(p), _stream(k_i8.device))
+        _lib.check(rc, "kv_append_paged", 1)
+    return q_out
+
+
+def kv_read_paged(k_i8, k_scale, v_i8, v_scale, block_table, context_lens, num_tokens, first=None, dtype=torch.float16):
+    """Tokens first[b] ... first[b] + num_tokens - 1 of every sequence as 16-bit (k, v) [B, H_kv, num_tokens, D]."""
+    what = "superl8_b200 kv_read_paged"
+    _check(dtype in (torch.float16, torch.bfloat16), f"{what}: dtype must be float16 or bfloat16")
+    if _compiled():
+        r = _ext.kv_read_paged(k_i8, k_scale, v_i8, v_scale, block_table, context_lens, int(num_tokens), first,
+                               dtype == torch.bfloat16)
+        _lib.launches += 1 if r[0].numel() else 0
+        return r
+    cache = _paged_cache(k_i8, k_scale, v_i8, v_scale, block_table, context_lens, what)
+    _check(0 <= int(num_tokens) <= 0x7fffffff, f"{what}: num_tokens must not be negative")
+    B = context_lens.shape[0]
+    start = _lens_ptr(first, k_i8, B, "first", what)
+    k = torch.empty((B, cache.Hkv, int(num_tokens), cache.D), dtype=dtype, device=k_i8.device)
+    v = torch.empty_like(k)
+    if k.numel():
+        with torch.cuda.device(k_i8.device):
+            rc = _lib.load().sl8_kv_read_paged(C.byref(cache), B, start, int(num_tokens), _DTYPE[dtype], k.data_ptr(),
+                                               v.data_ptr(), _stream(k_i8.device))
+        _lib.check(rc, "kv_read_paged", 1)
+    return k, v
+
+
+def attn_paged(q, k_i8, k_scale, v_i8, v_scale, block_table, context_lens, scale=None, causal=True, window_left=-1,
+               query_lens=None, max_context_len=0):
+    """Attention of q [B, H_q, M, D] over a paged int8 cache; output like q."""
+    what = "superl8_b200 attn_paged_cached"
+    window_left = -1 if window_left < 0 else min(int(window_left), 0x7fffffff)
+    limit = 0 if max_context_len is None else max(0, min(int(max_context_len), 0x7fffffff))
+    if _compiled():
+        r = _ext.attn_paged(q, k_i8, k_scale, v_i8, v_scale, block_table, context_lens, None if scale is None else float(scale),
+                            bool(causal), window_left, query_lens, limit)
+        _lib.launches += 2 if r.numel() else 0
+        return r
+    cache = _paged_cache(k_i8, k_scale, v_i8, v_scale, block_table, context_lens, what)
+    _on(q, k_i8, what)
+    _check(q.dtype in (torch.float16, torch.bfloat16), f"{what}: q must be float16 or bfloat16")
+    _check(q.dim() == 4, f"{what}: expect q [B,H,S,D]")
+    B, Hq, M, D = q.shape
+    _check(B == context_lens.shape[0] and D == cache.D, f"{what}: q must match the cache and block_table in batch and head dim")
+    _check(cache.Hkv > 0 and Hq % cache.Hkv == 0, f"{what}: H_q must be divisible by H_kv (GQA)")
+    qlens = _lens_ptr(query_lens, k_i8, B, "query_lens", what)
+    q = _rows(q, True)
+    out = torch.empty_like(q)
+    if out.numel() == 0:
+        return out
+    p = _lib.PagedAttnParams(q=q.data_ptr(), out=out.data_ptr(), **_steps(q, "q"), **_steps(out, "out"), query_lens=qlens, B=B,
+                             Hq=Hq, M=M, dtype=_DTYPE[q.dtype], causal=int(bool(causal)), window_left=window_left,
+                             max_context_len=limit, softmax_scale=(1.0 / math.sqrt(D)) if scale is None else float(scale))
+    lib = _lib.load()
+    with torch.cuda.device(q.device):
+        nbytes = int(lib.sl8_attn_paged_workspace(C.byref(cache), C.byref(p)))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        rc = lib.sl8_attn_paged(C.byref(cache), C.byref(p), _ptr(ws), nbytes, _stream(q.device))
+    _lib.check(rc, "attn_paged_cached", 2)
+    return out

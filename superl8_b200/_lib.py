@@ -117,7 +117,46 @@ class BwdParams(C.Structure):
     ]
 
 
-# name -> (restype, argtypes); every symbol declared in include/superl8_b200.h
+class RopeParams(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("q_out", C.c_void_p), ("k", C.c_void_p), ("k_out", C.c_void_p),
+        *[(f"{n}_stride_{d}", C.c_int64) for n in ("q", "q_out", "k", "k_out") for d in "bhs"],
+        ("positions", C.c_void_p), ("pos_stride_axis", C.c_int64), ("pos_stride_b", C.c_int64), ("pos_stride_s", C.c_int64),
+        ("inv_freq", C.c_void_p), ("freq_axis", C.c_void_p),
+        ("B", C.c_int32), ("Hq", C.c_int32), ("Hkv", C.c_int32), ("S", C.c_int32), ("D", C.c_int32), ("rot", C.c_int32),
+        ("dtype", C.c_int32), ("pos_is_64", C.c_int32), ("n_axes", C.c_int32), ("interleaved", C.c_int32), ("inverse", C.c_int32),
+    ]
+
+
+class PagedCache(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("block_table", C.c_void_p), ("table_stride", C.c_int64), ("context_lens", C.c_void_p),
+        ("num_pages", C.c_int32), ("Hkv", C.c_int32), ("page_size", C.c_int32), ("D", C.c_int32), ("max_pages", C.c_int32),
+    ]
+
+
+class AppendParams(C.Structure):
+    _fields_ = [
+        ("k_new", C.c_void_p), ("v_new", C.c_void_p), ("q", C.c_void_p), ("q_out", C.c_void_p),
+        *[(f"{n}_stride_{d}", C.c_int64) for n in ("k", "v", "q", "q_out") for d in "bhs"],
+        ("new_lens", C.c_void_p), ("positions", C.c_void_p), ("pos_stride_axis", C.c_int64), ("pos_stride_b", C.c_int64),
+        ("pos_stride_s", C.c_int64), ("inv_freq", C.c_void_p), ("freq_axis", C.c_void_p),
+        ("B", C.c_int32), ("Hq", C.c_int32), ("M", C.c_int32), ("rot", C.c_int32),
+        ("dtype", C.c_int32), ("pos_is_64", C.c_int32), ("n_axes", C.c_int32), ("interleaved", C.c_int32),
+    ]
+
+
+class PagedAttnParams(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("out", C.c_void_p), *[(f"{n}_stride_{d}", C.c_int64) for n in ("q", "out") for d in "bhs"],
+        ("query_lens", C.c_void_p), ("B", C.c_int32), ("Hq", C.c_int32), ("M", C.c_int32),
+        ("dtype", C.c_int32), ("causal", C.c_int32), ("window_left", C.c_int32), ("max_context_len", C.c_int32),
+        ("softmax_scale", C.c_float),
+    ]
+
+
+# name -> (restype, argtypes); every symbol declared in include/superl8_b200.h and superl8_b200_paged.h
 SIGNATURES = {
     "sl8_abi_version": (C.c_int, []),
     "sl8_status_string": (C.c_char_p, [C.c_int]),
@@ -163,6 +202,12 @@ SIGNATURES = {
     "sl8_quantize_v_perchannel": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_void_p,
                                             C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "sl8_attn_int8_decode_static": (C.c_int, [C.POINTER(DecodeParams), C.c_void_p, C.c_void_p]),
+    "sl8_rope": (C.c_int, [C.POINTER(RopeParams), C.c_void_p]),
+    "sl8_kv_append_paged": (C.c_int, [C.POINTER(PagedCache), C.POINTER(AppendParams), C.c_void_p]),
+    "sl8_kv_read_paged": (C.c_int, [C.POINTER(PagedCache), C.c_int32, C.c_void_p, C.c_int32, C.c_int, C.c_void_p, C.c_void_p,
+                                    C.c_void_p]),
+    "sl8_attn_paged_workspace": (C.c_size_t, [C.POINTER(PagedCache), C.POINTER(PagedAttnParams)]),
+    "sl8_attn_paged": (C.c_int, [C.POINTER(PagedCache), C.POINTER(PagedAttnParams), C.c_void_p, C.c_size_t, C.c_void_p]),
     "sl8_tensor_peak_probe": (C.c_int, [C.c_int, C.c_int, C.POINTER(C.c_double), C.c_void_p, C.c_size_t, C.c_void_p]),
     "sl8_tensor_peak_probe_n": (C.c_int, [C.c_int, C.c_int, C.c_int, C.POINTER(C.c_double), C.c_void_p, C.c_size_t, C.c_void_p]),
     "sl8_decode_static_status": (C.c_int, [C.c_void_p]),

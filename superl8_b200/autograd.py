@@ -97,3 +97,60 @@ def attn(q, k, v, *, causal: bool = False, scale: float | None = None):
 def attn_ref(q, k, v, *, causal: bool = False, scale: float | None = None):
     """Non-quantised attention sharing the analytic backward (reference superl8/autograd.py:106-108)."""
     return _AttnRef.apply(q, k, v, causal, scale)
+
+
+class _Rope(torch.autograd.Function):
+    """The rotation is linear and orthogonal: its gradient is the rotation by the opposite angle, itself
+    differentiable the same way."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, inv_freq, freq_axis, interleaved, inverse):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(positions, inv_freq, freq_axis)
+        ctx.interleaved, ctx.inverse = interleaved, inverse
+        return _C.rope(q, k, positions, inv_freq, freq_axis, interleaved, inverse)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        positions, inv_freq, freq_axis = ctx.saved_tensors
+        need_q, need_k = ctx.needs_input_grad[:2]
+        dq, dk = (dq if need_q else None), (dk if need_k else None)
+        if dq is None and dk is None:
+            return (None,) * 7
+        args = (positions, inv_freq, freq_axis, ctx.interleaved, not ctx.inverse)
+        first, second = (dq, dk) if dq is not None else (dk, None)
+        a, b = _Rope.apply(first, second, *args)
+        return (a, b, None, None, None, None, None) if dq is not None else (None, a, None, None, None, None, None)
+
+
+def apply_rope(q, k, positions, inv_freq, *, freq_axis=None, interleaved: bool = False):
+    """Rotary positions on q [B, Hq, S, D] and k [B, Hkv, S, D] (``k`` may be None): (q_out, k_out).
+
+    Channel pair i of a row turns by ``positions[axis(i)] * inv_freq[i]``: pairs are channels
+    (i, i + rot/2) with rot = 2 len(inv_freq), or (2i, 2i + 1) with ``interleaved``; channels from rot on
+    stay.  ``positions``: int32 / int64 [S], [B, S], or [axes, B, S] with ``freq_axis`` (uint8 [rot/2])
+    naming the axis of every frequency -- time, height and width for images and video (see
+    :func:`rope_freq_axis`).  fp16 / bf16 / fp32, any even D, strided views with contiguous channels in
+    place.  Angles are formed in 64 bits, so far positions keep their precision.  Differentiable in q and
+    k (also twice); ``inv_freq`` is a constant.  What it returns is what ``attn``, ``attn_int8_fwd`` and the
+    other prefill operators take; ``kv_append_paged`` does the same rotation on the way into a cache."""
+    if inv_freq.requires_grad:
+        raise RuntimeError("superl8_b200 apply_rope: inv_freq is a constant (no gradient is computed for it)")
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _Rope.apply(q, k, positions, inv_freq, freq_axis, bool(interleaved), False)
+    return _C.rope(q, k, positions, inv_freq, freq_axis, interleaved)
+
+
+def rope_freq_axis(sections, *, mixed: bool = False, device=None) -> torch.Tensor:
+    """uint8 [sum(sections)]: the axis of every frequency when axis a owns ``sections[a]`` of them -- in
+    blocks (all of axis 0, then axis 1, ...), or ``mixed``: dealt out in turn (0, 1, 2, 0, 1, 2, ...)
+    until an axis has its share."""
+    sections = [int(n) for n in sections]
+    if not sections or len(sections) > 255 or min(sections) < 0:
+        raise ValueError("superl8_b200 rope_freq_axis: sections must be 1 to 255 numbers >= 0")
+    if mixed:
+        order = sorted((i, a) for a, n in enumerate(sections) for i in range(n))
+        axis = [a for _, a in order]
+    else:
+        axis = [a for a, n in enumerate(sections) for _ in range(n)]
+    return torch.tensor(axis, dtype=torch.uint8, device=device)

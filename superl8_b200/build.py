@@ -40,7 +40,7 @@ def _nvcc() -> str:
 
 
 def _newest_header_mtime() -> float:
-    hdrs = list(CSRC.glob("*.cuh")) + [PKG_DIR.parent / "include" / "superl8_b200.h"]
+    hdrs = list(CSRC.glob("*.cuh")) + list((PKG_DIR.parent / "include").glob("*.h"))
     return max(h.stat().st_mtime for h in hdrs if h.exists())
 
 
@@ -85,7 +85,7 @@ def build(force: bool = False, verbose: bool = False, trace: bool = False, defin
     return lib_path
 
 
-EXT_SRC = CSRC / "torch_ext" / "sl8_torch_ext.cpp"
+EXT_SRCS = sorted((CSRC / "torch_ext").glob("*.cpp"))
 EXT_NAME = "_C_ext"
 
 
@@ -95,7 +95,7 @@ def ext_path() -> Path:
 
 
 def build_torch_ext(force: bool = False) -> Path:
-    """Compiles the thin torch extension (csrc/torch_ext) with g++ against the installed torch and
+    """Compiles the thin torch extension (csrc/torch_ext/*.cpp) with g++ against the installed torch and
     links it to libsuperl8_b200.so; the result sits beside the library (in-tree, nothing goes to a
     JIT cache).  Needs no GPU and no nvcc, only the CUDA headers torch's own headers include."""
     import sysconfig
@@ -104,23 +104,30 @@ def build_torch_ext(force: bool = False) -> Path:
     from torch.utils import cpp_extension as ce
 
     out = ext_path()
-    hdr = PKG_DIR.parent / "include" / "superl8_b200.h"
-    if out.exists() and not force and out.stat().st_mtime > max(EXT_SRC.stat().st_mtime, hdr.stat().st_mtime):
+    newest = max(h.stat().st_mtime for h in [*EXT_SRCS, *(PKG_DIR.parent / "include").glob("*.h")])
+    if out.exists() and not force and out.stat().st_mtime > newest:
         return out
     build()  # the extension links against the library
     cuda_home = os.environ.get("CUDA_HOME") or "/usr/local/cuda"
     incs = [*ce.include_paths(), sysconfig.get_paths()["include"], str(Path(cuda_home) / "include")]
     torch_lib = str(Path(torch.__file__).resolve().parent / "lib")
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-DTORCH_EXTENSION_NAME={EXT_NAME}", "-DTORCH_API_INCLUDE_EXTENSION_H",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *[f"-I{i}" for i in incs], str(EXT_SRC), "-o", str(out),
+    cxx = os.environ.get("CXX", "g++")
+    objs = [BUILD_DIR / ("ext_" + src.stem + ".o") for src in EXT_SRCS]
+
+    def run(cmd):
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError("torch extension build failed: " + " ".join(cmd) + "\n" + r.stdout + r.stderr)
+
+    with ThreadPoolExecutor(max_workers=len(objs)) as ex:
+        list(ex.map(lambda so: run([cxx, "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
+                                    f"-DTORCH_EXTENSION_NAME={EXT_NAME}", "-DTORCH_API_INCLUDE_EXTENSION_H",
+                                    f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                                    *[f"-I{i}" for i in incs], "-c", str(so[0]), "-o", str(so[1])]), zip(EXT_SRCS, objs)))
+    run([cxx, "-shared", *map(str, objs), "-o", str(out),
            f"-L{torch_lib}", f"-L{PKG_DIR}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python",
            "-l:libsuperl8_b200.so",
-           "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError("torch extension build failed: " + " ".join(cmd) + "\n" + r.stdout + r.stderr)
+           "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"])
     return out
 
 

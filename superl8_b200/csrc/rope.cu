@@ -1,0 +1,151 @@
+// Rotary positions with one or several axes on q and k (one launch for both), and the gradient,
+// which is the rotation by the opposite angle.
+//
+// HBM bound: every element is read once and written once, 2 e bytes.  A thread owns one item -- 2 VEC
+// channels of one token that pair with one another -- works out its VEC angles once and walks the
+// heads with them, so the angles (64-bit products, sincospif) are shared by all heads of a block's
+// group and the loads of four heads are in flight together.
+#include "sl8_rope.cuh"
+
+namespace sl8 {
+namespace {
+
+struct RopeTensor {
+  const void* x;
+  void* y;
+  int64_t x_sb, x_sh, x_ss, y_sb, y_sh, y_ss;
+};
+
+struct RopeArgs {
+  RopeTensor q, k;
+  RopeFreq f;
+  int64_t tokens;   // B * S
+  int S, Hq, H, items, heads_per_block, interleaved;   // H = Hq + Hkv
+};
+
+constexpr int kRopeThreads = 256;
+constexpr int kRopeUnroll = 4;
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
+  const int64_t item = (int64_t)blockIdx.x * kRopeThreads + threadIdx.x;
+  const int64_t token = item / a.items;
+  if (token >= a.tokens) return;
+  const int j = (int)(item - token * a.items);
+  const int64_t b = token / a.S, s = token - b * a.S;
+  const bool turn = j * VEC < a.f.half;
+  const int2 at = rope_item<VEC>(j, a.f.half, a.interleaved != 0);
+  const int h0 = blockIdx.y * a.heads_per_block, h1 = min(a.H, h0 + a.heads_per_block);
+
+  Piece<T, VEC> p0[kRopeUnroll], p1[kRopeUnroll];
+  auto load = [&](int h, Piece<T, VEC>& u, Piece<T, VEC>& w) {
+    const RopeTensor& t = h < a.Hq ? a.q : a.k;
+    const T* x = reinterpret_cast<const T*>(t.x) + b * t.x_sb + (h < a.Hq ? h : h - a.Hq) * t.x_sh + s * t.x_ss;
+    u = piece_load<T, VEC>(x + at.x);
+    w = piece_load<T, VEC>(x + at.y);
+  };
+  auto store = [&](int h, const Piece<T, VEC>& u, const Piece<T, VEC>& w) {
+    const RopeTensor& t = h < a.Hq ? a.q : a.k;
+    T* y = reinterpret_cast<T*>(t.y) + b * t.y_sb + (h < a.Hq ? h : h - a.Hq) * t.y_sh + s * t.y_ss;
+    *reinterpret_cast<Piece<T, VEC>*>(y + at.x) = u;
+    *reinterpret_cast<Piece<T, VEC>*>(y + at.y) = w;
+  };
+  // the first heads' loads go out before the angles are worked out
+#pragma unroll
+  for (int i = 0; i < kRopeUnroll; ++i)
+    if (h0 + i < h1) load(h0 + i, p0[i], p1[i]);
+  float c[VEC], sn[VEC];
+  if (turn) rope_angles<VEC>(a.f, j * VEC, b, s, c, sn);
+  for (int h = h0; h < h1; h += kRopeUnroll) {
+    if (h != h0) {
+#pragma unroll
+      for (int i = 0; i < kRopeUnroll; ++i)
+        if (h + i < h1) load(h + i, p0[i], p1[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kRopeUnroll; ++i) {
+      if (h + i < h1) {
+        if (turn) {
+          float u[VEC], w[VEC];
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) { u[e] = to_f32<T>(p0[i].v[e]); w[e] = to_f32<T>(p1[i].v[e]); }
+          rope_turn<VEC>(u, w, c, sn, a.interleaved != 0);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) { p0[i].v[e] = from_f32<T>(u[e]); p1[i].v[e] = from_f32<T>(w[e]); }
+        }
+        store(h + i, p0[i], p1[i]);
+      }
+    }
+  }
+}
+
+template <typename T, int VEC>
+int launch_rope(RopeArgs a, int D, cudaStream_t stream) {
+  a.items = D / (2 * VEC);
+  const int64_t gx = (a.tokens * a.items + kRopeThreads - 1) / kRopeThreads;
+  if (gx > 0x7fffffffll) return SL8_ERR_TOO_LARGE;
+  // As many heads per block as still leave eight blocks per SM: the angles are worked out once per block.
+  int64_t groups = (kNumSms * 8 + gx - 1) / gx;
+  if (groups > a.H) groups = a.H;
+  a.heads_per_block = (int)((a.H + groups - 1) / groups);
+  const unsigned gy = (unsigned)((a.H + a.heads_per_block - 1) / a.heads_per_block);
+  if (gy > 65535u) return SL8_ERR_TOO_LARGE;
+  rope_kernel<T, VEC><<<dim3((unsigned)gx, gy), kRopeThreads, 0, stream>>>(a);
+  return cudaGetLastError() == cudaSuccess ? SL8_OK : SL8_ERR_CUDA;
+}
+
+template <typename T>
+int launch_rope_vec(const RopeArgs& a, int D, int vec, cudaStream_t stream) {
+  switch (vec) {
+    case 8: return launch_rope<T, 8>(a, D, stream);
+    case 4: return launch_rope<T, 4>(a, D, stream);
+    case 2: return launch_rope<T, 2>(a, D, stream);
+    default: return launch_rope<T, 1>(a, D, stream);
+  }
+}
+
+// Largest piece (elements) that keeps every row's pieces whole and aligned.
+int piece_size(const sl8_rope_params& p, int elem) {
+  for (int vec = 8; vec > 1; vec /= 2) {
+    const int64_t bytes = (int64_t)vec * elem > 16 ? 16 : (int64_t)vec * elem;
+    bool ok = (p.rot / 2) % vec == 0 && p.D % (2 * vec) == 0;
+    auto fits = [&](const void* x, int64_t sb, int64_t sh, int64_t ss) {
+      return x == nullptr || (reinterpret_cast<uintptr_t>(x) % bytes == 0 && sb * elem % bytes == 0 && sh * elem % bytes == 0 &&
+                              ss * elem % bytes == 0);
+    };
+    ok = ok && fits(p.q, p.q_stride_b, p.q_stride_h, p.q_stride_s) && fits(p.q_out, p.q_out_stride_b, p.q_out_stride_h, p.q_out_stride_s) &&
+         fits(p.k, p.k_stride_b, p.k_stride_h, p.k_stride_s) && fits(p.k_out, p.k_out_stride_b, p.k_out_stride_h, p.k_out_stride_s);
+    if (ok) return vec;
+  }
+  return 1;
+}
+
+}  // namespace
+}  // namespace sl8
+
+using namespace sl8;
+
+extern "C" int sl8_rope(const sl8_rope_params* p, void* stream) {
+  if (p == nullptr) return SL8_ERR_NULL;
+  if (p->B < 0 || p->Hq < 0 || p->Hkv < 0 || p->S < 0 || p->n_axes < 1) return SL8_ERR_BAD_SHAPE;
+  if (p->D < 2 || p->D % 2 != 0 || p->rot < 0 || p->rot > p->D || p->rot % 2 != 0) return SL8_ERR_BAD_SHAPE;
+  if (p->dtype != SL8_F16 && p->dtype != SL8_BF16 && p->dtype != SL8_F32) return SL8_ERR_BAD_DTYPE;
+  const int Hq = p->q ? p->Hq : 0, Hkv = p->k ? p->Hkv : 0;
+  if ((int64_t)p->B * p->S * (Hq + Hkv) == 0) return SL8_OK;
+  if ((Hq && !p->q_out) || (Hkv && !p->k_out) || !p->positions || (p->rot > 0 && !p->inv_freq)) return SL8_ERR_NULL;
+  const int elem = p->dtype == SL8_F32 ? 4 : 2;
+  RopeArgs a{};
+  a.q = RopeTensor{p->q, p->q_out, p->q_stride_b, p->q_stride_h, p->q_stride_s, p->q_out_stride_b, p->q_out_stride_h, p->q_out_stride_s};
+  a.k = RopeTensor{p->k, p->k_out, p->k_stride_b, p->k_stride_h, p->k_stride_s, p->k_out_stride_b, p->k_out_stride_h, p->k_out_stride_s};
+  a.f = RopeFreq{p->positions, p->pos_stride_axis, p->pos_stride_b, p->pos_stride_s, p->inv_freq, p->n_axes > 1 ? p->freq_axis : nullptr,
+                 p->pos_is_64 != 0, p->n_axes, p->rot / 2, p->inverse ? -1.f : 1.f};
+  a.tokens = (int64_t)p->B * p->S;
+  a.S = p->S; a.Hq = Hq; a.H = Hq + Hkv; a.interleaved = p->interleaved;
+  const int vec = piece_size(*p, elem);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (p->dtype) {
+    case SL8_F16: return launch_rope_vec<__half>(a, p->D, vec, s);
+    case SL8_BF16: return launch_rope_vec<__nv_bfloat16>(a, p->D, vec, s);
+    default: return launch_rope_vec<float>(a, p->D, vec, s);
+  }
+}

@@ -344,6 +344,8 @@ int64_t device_status(const Tensor& like) {
 
 }  // namespace
 
+void bind_paged(pybind11::module_& m);   // sl8_torch_paged.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "superl8_b200: the reference's compiled operators for the int8 attention path, over libsuperl8_b200.so";
   m.def("quantize_i8_rowwise", &quantize_i8_rowwise, py::arg("x"));
@@ -362,4 +364,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attn_int8_prefill", &attn_int8_prefill, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("causal") = false,
         py::arg("scale") = 0.0, py::arg("window_left") = -1, py::arg("gate") = true, py::arg("ask_first") = false);
   m.def("device_status", &device_status, py::arg("like"));
+  bind_paged(m);
 }
