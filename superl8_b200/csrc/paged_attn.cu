@@ -10,10 +10,10 @@
 // matter), so K's codes enter the integer MMA as they lie in memory and only V's are widened.
 //
 // What bounds it: HBM, 2 D bytes per key and KV head.  All query rows that share a KV head (the GQA group
-// times the query tokens) are served by one pass over its keys, with keys on the M axis of the MMA (16 per
-// warp and step) and 8 query rows on the N axis, so a group of 8 heads wastes nothing.  Every warp streams
-// its own 16-key chunks (a chunk never crosses a page: page sizes are multiples of 16) through a private
-// ring of cp.async stages: no barrier inside the loop, 160 KB in flight per SM.
+// times the query tokens) are served by one pass over its keys, with keys on the M axis of the MMA (tiles
+// of 16) and 8 query rows on the N axis, so a group of 8 heads wastes nothing.  Every warp streams
+// its own chunks of 32 or 16 keys (a 16-key tile never crosses a page: page sizes are multiples of 16) through
+// a private ring of cp.async stages: no barrier inside the loop, 128 KB in flight per SM.
 //
 // Split.  The chunks of all (sequence, KV head) units form one line, cut into equal ranges, one per block
 // of a one-block-per-SM grid, whatever the lengths are; a unit that lies in one range is finished there,
@@ -29,7 +29,6 @@ namespace {
 
 constexpr int kPaWarps = 8;
 constexpr int kPaThreads = 32 * kPaWarps;
-constexpr int kChunk = 16;      // keys per warp and step
 
 struct PagedArgs {
   const void* q;
@@ -47,13 +46,14 @@ struct PagedArgs {
   int B, Hq, Hkv, M, G, rows;              // rows = M * G query rows per (sequence, KV head)
   int page_shift, num_pages, max_pages;
   int causal, window, bf16;
-  int row_warps;      // warps that share a key but hold other rows (1, 2, 4)
+  int row_warps;      // warps that share a key but hold other rows (1 or 2)
   int rows_per_unit, row_units;            // rows = up to row_units * rows_per_unit
   int blocks;         // blocks of the split kernel
+  int chunk_shift;    // log2 of the keys per warp and step
   float scale_log2;   // softmax_scale * log2 e
 };
 
-// What a sequence asks for: tokens that exist, its query tokens, the first 16-key chunk a query can see.
+// What a sequence asks for: tokens that exist, its query tokens, the first chunk a query can see.
 struct Seq {
   int len, n, first_chunk, chunks;
   int place;   // of query token 0
@@ -68,44 +68,49 @@ __device__ __forceinline__ Seq seq_of(const PagedArgs& a, int b) {
   s.place = max(context, 0) - s.n;
   int64_t lo = 0;
   if (a.window >= 0) lo = max((int64_t)0, (int64_t)s.place - a.window + 1);
-  s.first_chunk = (int)(lo / kChunk);
-  s.chunks = (s.n > 0 && lo < s.len) ? (s.len + kChunk - 1) / kChunk - s.first_chunk : 0;
+  s.first_chunk = (int)(lo >> a.chunk_shift);
+  s.chunks = (s.n > 0 && lo < s.len) ? (int)(((int64_t)s.len + (1 << a.chunk_shift) - 1) >> a.chunk_shift) - s.first_chunk : 0;
   return s;
 }
 
-// Block-wide: chunks of all units together, and those of the sequences before `upto`.
-// `find` >= 0 (a place on the line) also yields the sequence that holds it.
+// The line: the chunks of all units, sequence by sequence (the host bounds it below 2^31).  Every thread owns
+// a run of ceil(B / threads) sequences; returns the line's length and the place where the run begins.
 struct Line {
-  long long total, before;
-  int b;   // sequence that holds `find`
+  unsigned total, begin;
+  int b0, b1;
 };
 
-__device__ Line line_of(const PagedArgs& a, int upto, int units, long long (*red)[2]) {
+__device__ Line line_of(const PagedArgs& a, int units, unsigned* red) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  long long sum = 0, pre = 0;
-  for (int b = tid; b < a.B; b += kPaThreads) {
-    const long long c = seq_of(a, b).chunks;
-    sum += c;
-    if (b < upto) pre += c;
-  }
+  const int run = (a.B + kPaThreads - 1) / kPaThreads;
+  Line l;
+  l.b0 = min(a.B, tid * run);
+  l.b1 = min(a.B, l.b0 + run);
+  unsigned own = 0;
+  for (int b = l.b0; b < l.b1; ++b) own += seq_of(a, b).chunks;
+  own *= units;
+  unsigned inc = own;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    pre += __shfl_xor_sync(0xffffffffu, pre, o);
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned up = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += up;
   }
-  if (lane == 0) { red[warp][0] = sum; red[warp][1] = pre; }
+  if (lane == 31) red[warp] = inc;
   __syncthreads();
-  Line l{0, 0, 0};
-  for (int w = 0; w < kPaWarps; ++w) { l.total += red[w][0]; l.before += red[w][1]; }
-  l.total *= units;
-  l.before *= units;
+  l.total = 0;
+  l.begin = inc - own;
+#pragma unroll
+  for (int w = 0; w < kPaWarps; ++w) {
+    if (w == warp) l.begin += l.total;
+    l.total += red[w];
+  }
   return l;
 }
 
 // Chunks per block: equal shares, whole rounds of the block's warps.
-__device__ __forceinline__ long long share_of(long long total, int blocks) {
-  const long long per = (total + blocks - 1) / blocks;
-  return max((long long)kPaWarps, (per + kPaWarps - 1) / kPaWarps * kPaWarps);
+__device__ __forceinline__ unsigned share_of(unsigned total, int blocks) {
+  const unsigned per = (total + blocks - 1) / blocks;
+  return max((unsigned)kPaWarps, (per + kPaWarps - 1) / kPaWarps * kPaWarps);
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
@@ -123,6 +128,16 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
+__device__ __forceinline__ float lg2_approx(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 // 16-byte piece `c` of row `r` of a [16][D] byte tile: pieces are exchanged within 128 bytes so that the
 // eight rows of an ldmatrix lie in eight different bank groups.
@@ -133,25 +148,42 @@ __device__ __forceinline__ uint32_t tile_offset(int r, int c) {
   return r * D + ((c ^ ((r >> SH) & MASK)) << 4);
 }
 
+// Keys per warp and step: 32 (two 16-key tiles share the maximum, the rescaling and the loop) where the
+// accumulators leave the registers for it and the ring the space, else 16.
+__host__ __device__ constexpr int chunk_shift_of(int D, int ng) { return D == 256 || (D >= 64 && ng == 4) ? 4 : 5; }
+
+// Most groups of 8 query rows a warp can accumulate: D / 4 registers a thread each.
+__host__ __device__ constexpr int groups_of(int D) { return D == 256 ? 2 : 4; }
+
 template <int D, int NG>
 struct PaCfg {
-  static constexpr int SLOT = 2 * kChunk * D + 16;                       // K rows, V rows, the two scales
-  static constexpr int STAGES = D == 256 ? 2 : (D == 128 ? 5 : (D == 64 ? 10 : 16));
+  static constexpr int SHIFT = chunk_shift_of(D, NG);
+  static constexpr int TILES = (1 << SHIFT) / 16;                        // 16-key tiles per chunk
+  static constexpr int TILE = 2 * 16 * D + 16;                           // K rows, V rows, the two scales
+  static constexpr int SLOT = TILES * TILE;
+  static constexpr int STAGES = D == 256 ? 2 : (D == 128 ? (TILES == 2 ? 3 : 5) : (D == 64 ? (TILES == 2 ? 5 : 10) : 8));
   static constexpr int RING = kPaWarps * STAGES * SLOT;
-  static constexpr int BUF_ROW = D + 8;                                  // floats per row of the merge buffer
+  static constexpr int JOIN = D >= 128 ? D / 2 : D;                      // channels joined at a time
+  static constexpr int BUF_ROW = JOIN + 8;                               // floats per row of the joining buffer
   static constexpr int BUF = kPaWarps * 8 * BUF_ROW * 4;
   static constexpr int Q_GROUP = D * 16;                                 // two int8 planes of 8 rows, fragment order
   static constexpr int ML = kPaWarps * NG * 8 * 8;
-  static constexpr int GROUPS = D == 256 ? 4 : 8;                        // row groups of 8 a block may hold
+  static constexpr int ROW_WARPS = NG == groups_of(D) ? 2 : 1;           // most warps with rows of their own
+  static constexpr bool Q_REGS = NG * D <= 256;                          // fragments of Q held in registers
   static constexpr int smem(int row_warps) { return RING + BUF + ML + row_warps * NG * (Q_GROUP + 32); }
-  static_assert(smem(GROUPS / NG) <= 226 * 1024, "over the shared memory of an SM");
+  static_assert(smem(ROW_WARPS) <= 226 * 1024, "over the shared memory of an SM");
 };
+
+// A row's reference M moves only when a logit passes it by this much (in powers of two): the weights stay
+// below 2^8, far inside fp16, and the accumulators are hardly ever rescaled.
+constexpr float kSlack = 8.f;
 
 template <int D, int NG>
 __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedArgs a) {
   using C = PaCfg<D, NG>;
+  constexpr int T = C::TILES, KEYS = 1 << C::SHIFT;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ long long red[kPaWarps][2];
+  __shared__ unsigned red[kPaWarps];
   __shared__ int s_start[3];
   float* buf = reinterpret_cast<float*>(smem + C::RING);
   float2* ml = reinterpret_cast<float2*>(smem + C::RING + C::BUF);       // [warp][NG * 8]
@@ -165,44 +197,33 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
   const int units = a.Hkv * a.row_units;                                 // of one sequence
 
   // ---- this block's range of the line ----
-  const Line line = line_of(a, 0, units, red);
-  const long long per = share_of(line.total, a.blocks);
-  const long long c0 = per * blockIdx.x;
-  const long long c1 = min(line.total, c0 + per);
+  const Line line = line_of(a, units, red);
+  const unsigned per = share_of(line.total, a.blocks);
+  const unsigned c0 = min(line.total, per * blockIdx.x);
+  const unsigned c1 = min(line.total, c0 + per);
   if (c0 >= c1) return;
-  if (warp == 0) {
-    // the sequence that holds c0: a warp walks the batch 32 at a time
-    long long at = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 32) {
-      const int b = b0 + lane;
-      const long long own = b < a.B ? (long long)seq_of(a, b).chunks * units : 0;
-      long long inc = own;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += up;
-      }
-      const long long begin = at + inc - own;
-      if (own > 0 && begin <= c0 && c0 < begin + own) {
-        const int chunks = (int)(own / units);
+  if (line.begin <= c0) {
+    unsigned at = line.begin;
+    for (int b = line.b0; b < line.b1; ++b) {
+      const unsigned chunks = seq_of(a, b).chunks, own = chunks * units;
+      if (c0 >= at && c0 - at < own) {
         s_start[0] = b;
-        s_start[1] = (int)((c0 - begin) / chunks);
-        s_start[2] = (int)((c0 - begin) % chunks);
+        s_start[1] = (int)((c0 - at) / chunks);
+        s_start[2] = (int)((c0 - at) % chunks);
       }
-      at += __shfl_sync(0xffffffffu, inc, 31);
-      if (at > c0) break;
+      at += own;
     }
   }
   __syncthreads();
 
-  // ---- the loads' cursor: this warp's next chunk, running ahead of the compute cursor ----
+  // ---- the two cursors of a warp: compute, and the loads that run ahead of it across units ----
   struct Cursor {
     int b, u, c, cend;
-    long long left;    // chunks of the block's range behind this segment
+    int left;          // chunks of the block's range behind this segment
     Seq s;
   };
   auto open = [&](Cursor& x, int c_begin) {
-    x.cend = (int)min((long long)x.s.chunks, c_begin + x.left);
+    x.cend = min(x.s.chunks, c_begin + x.left);
     x.left -= x.cend - c_begin;
     x.c = c_begin + kw;
   };
@@ -216,56 +237,70 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
   Cursor cur;
   cur.b = s_start[0]; cur.u = s_start[1];
   cur.s = seq_of(a, cur.b);
-  cur.left = c1 - c0;
+  cur.left = (int)(c1 - c0);
   int c_begin = s_start[2];
   open(cur, c_begin);
 
   uint8_t* ring = smem + warp * C::STAGES * C::SLOT;
   const uint32_t ring_addr = smem_u32(ring);
+  // Loads of a chunk: a half-warp per tile when there are two (each tile has its own page), else the warp.
+  constexpr int LANES = 32 / T;                       // lanes that load one tile
+  const int l_tile = T == 2 ? lane >> 4 : 0, l_lane = lane & (LANES - 1);
+  const uint32_t l_dst = ring_addr + l_tile * C::TILE;
   Cursor ahead = cur;
-  bool more = true;
-  int page = -1;
-  auto find_page = [&]() {   // the page of the cursor's chunk, asked for one step before it is needed
-    while (ahead.c >= ahead.cend) {
-      if (ahead.left <= 0) { more = false; return; }
-      next_unit(ahead);
-    }
-    page = __ldg(a.table + ahead.b * a.table_stride + ((int64_t)(ahead.s.first_chunk + ahead.c) * kChunk >> a.page_shift));
+  const int32_t* a_row = a.table + ahead.b * a.table_stride;
+  int a_head = ahead.u / a.row_units;
+  int a_tok = 0, page = -1;
+  const int page_mask = (1 << a.page_shift) - 1;
+  auto find_page = [&]() {   // the page of this lane's tile, asked for one step before it is needed
+    a_tok = (ahead.s.first_chunk + ahead.c) * KEYS + 16 * l_tile;
+    page = a_tok < ahead.s.len ? __ldg(a_row + (a_tok >> a.page_shift)) : -1;
   };
-  find_page();
+  auto seek = [&]() {        // the next segment with a chunk for this warp; none: c stays at or past cend
+    while (ahead.c >= ahead.cend && ahead.left > 0) {
+      next_unit(ahead);
+      a_row = a.table + ahead.b * a.table_stride;
+      a_head = ahead.u / a.row_units;
+    }
+    if (ahead.c < ahead.cend) find_page();
+  };
+  seek();
   auto issue = [&](int slot) {
-    if (more) {
-      const bool held = page >= 0 && page < a.num_pages;   // otherwise zeros, and a scale of 0: nothing is seen
-      const int64_t ph = held ? (int64_t)page * a.Hkv + ahead.u / a.row_units : 0;
-      const int in_page = ((ahead.s.first_chunk + ahead.c) * kChunk) & ((1 << a.page_shift) - 1);
-      const int64_t at = ((ph << a.page_shift) + (held ? in_page : 0)) * D;
-      const uint32_t dst = ring_addr + slot * C::SLOT;
-      const int n16 = held ? 16 : 0, n4 = held ? 4 : 0;
+    if (ahead.c < ahead.cend) {
+      const bool held = (unsigned)page < (unsigned)a.num_pages;   // otherwise zeros, and a scale of 0: nothing is seen
+      const int64_t ph = held ? (int64_t)page * a.Hkv + a_head : 0;
+      const int64_t at = held ? ((ph << a.page_shift) + (a_tok & page_mask)) * D + 16 * l_lane : 0;
+      const uint32_t dst = l_dst + slot * C::SLOT;
+      const int n16 = held ? 16 : 0;
+      const int8_t* ksrc = a.k + at;
+      const int8_t* vsrc = a.v + at;
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        const int idx = lane + 32 * i, r = idx / (D / 16), c = idx % (D / 16);
-        cp_async16(dst + tile_offset<D>(r, c), a.k + at + 16 * idx, n16);
+      for (int i = 0; i < D / LANES; ++i) {
+        const int idx = l_lane + LANES * i;
+        cp_async16(dst + tile_offset<D>(idx / (D / 16), idx % (D / 16)), ksrc + 16 * LANES * i, n16);
       }
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        const int idx = lane + 32 * i, r = idx / (D / 16), c = idx % (D / 16);
-        cp_async16(dst + kChunk * D + tile_offset<D>(r, c), a.v + at + 16 * idx, n16);
+      for (int i = 0; i < D / LANES; ++i) {
+        const int idx = l_lane + LANES * i;
+        cp_async16(dst + 16 * D + tile_offset<D>(idx / (D / 16), idx % (D / 16)), vsrc + 16 * LANES * i, n16);
       }
-      if (lane < 2) cp_async4(dst + 2 * kChunk * D + 4 * lane, (lane ? a.vs : a.ks) + ph, n4);
+      if (l_lane < 2) cp_async4(dst + 32 * D + 4 * l_lane, (l_lane ? a.vs : a.ks) + ph, held ? 4 : 0);
       ahead.c += key_warps;
-      find_page();
+      if (ahead.c < ahead.cend) find_page(); else seek();
     }
     cp_async_commit();
   };
-  int slot_in = 0, slot_out = 0;
 #pragma unroll 1
   for (int i = 0; i < C::STAGES - 1; ++i) issue(i);
-  slot_in = C::STAGES - 1;
+  int slot_in = C::STAGES - 1, slot_out = 0;
+
+  // ldmatrix rows and pieces of this lane: K tiles [key][channel] and, transposing, V
+  const int m_row = (lane & 7) + ((lane >> 3) & 1) * 8, m_piece = lane >> 4;
 
   float o[NG][D / 16][4];
   while (true) {
     // ================= one segment: chunks [c_begin, cur.cend) of unit (cur.b, cur.u) =================
-    const int hkv = cur.u / a.row_units, row0 = (cur.u % a.row_units) * a.rows_per_unit;
+    const int hkv = cur.u / a.row_units, row0 = (cur.u - hkv * a.row_units) * a.rows_per_unit;
     const Seq s = cur.s;
     // ---- Q of the segment: two int8 planes in fragment order ----
     for (int grp = warp; grp < a.row_warps * NG; grp += kPaWarps) {
@@ -273,25 +308,27 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
       const int i = r / a.G, head = hkv * a.G + r % a.G;
       const bool live = r < a.rows && i < s.n;
       const uint2* src = reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(a.q) + cur.b * a.q_sb + head * a.q_sh + i * a.q_ss);
+      uint2 raw[D / 32][2];
+#pragma unroll
+      for (int w = 0; w < D / 32; ++w)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) raw[w][h] = live ? __ldg(src + 8 * w + 4 * h + t) : make_uint2(0, 0);
       float x[D / 32][2][4];
-      float top = 0.f;
+      uint32_t bits = 0;   // the largest magnitude, compared as bits: a NaN stays the largest
 #pragma unroll
       for (int w = 0; w < D / 32; ++w) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint2 p = live ? __ldg(src + 8 * w + 4 * h + t) : make_uint2(0, 0);
-          const float2 u0 = a.bf16 ? unpack2<__nv_bfloat16>(p.x) : unpack2<__half>(p.x);
-          const float2 u1 = a.bf16 ? unpack2<__nv_bfloat16>(p.y) : unpack2<__half>(p.y);
+          const float2 u0 = a.bf16 ? unpack2<__nv_bfloat16>(raw[w][h].x) : unpack2<__half>(raw[w][h].x);
+          const float2 u1 = a.bf16 ? unpack2<__nv_bfloat16>(raw[w][h].y) : unpack2<__half>(raw[w][h].y);
           x[w][h][0] = u0.x; x[w][h][1] = u0.y; x[w][h][2] = u1.x; x[w][h][3] = u1.y;
 #pragma unroll
-          for (int e = 0; e < 4; ++e)   // as bits: a NaN stays the largest
-            top = __uint_as_float(max(__float_as_uint(top), __float_as_uint(x[w][h][e]) & 0x7fffffffu));
+          for (int e = 0; e < 4; ++e) bits = max(bits, __float_as_uint(x[w][h][e]) & 0x7fffffffu);
         }
       }
-      uint32_t bits = __float_as_uint(top);
       bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
       bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 2));
-      top = __uint_as_float(bits);
+      const float top = __uint_as_float(bits);
       const float inv = top < 1e-30f ? 0.f : 16256.f / top;   // a row of zeros has logits of zero
 #pragma unroll
       for (int w = 0; w < D / 32; ++w) {
@@ -313,18 +350,23 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
 
     // ---- the segment's rows of this warp ----
     float row_scale[NG][2], m_run[NG][2], l_run[NG][2];
+    uint4 qr[C::Q_REGS ? NG : 1][C::Q_REGS ? D / 32 : 1];
+    const uint4* my_q = qf + rw * NG * (D / 32) * 32 + lane;
 #pragma unroll
-    for (int ng = 0; ng < NG; ++ng)
+    for (int ng = 0; ng < NG; ++ng) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         row_scale[ng][e] = qs[(rw * NG + ng) * 8 + 2 * t + e];
         m_run[ng][e] = kNegSentinel;
         l_run[ng][e] = 0.f;
       }
+      if constexpr (C::Q_REGS) {
 #pragma unroll
-    for (int ng = 0; ng < NG; ++ng)
+        for (int w = 0; w < D / 32; ++w) qr[ng][w] = my_q[(ng * (D / 32) + w) * 32];
+      }
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) o[ng][d][0] = o[ng][d][1] = o[ng][d][2] = o[ng][d][3] = 0.f;
+    }
     // keys every valid row of the warp sees: [all_from, all_to)
     const int r_first = row0 + rw * NG * 8;
     const int i_first = r_first / a.G, i_last = min(s.n, (min(a.rows, r_first + NG * 8) - 1) / a.G + 1) - 1;
@@ -336,52 +378,73 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
       slot_in = slot_in + 1 == C::STAGES ? 0 : slot_in + 1;
       cp_async_wait<C::STAGES - 1>();
       __syncwarp();
-      const uint32_t kbase = ring_addr + slot_out * C::SLOT, vbase = kbase + kChunk * D;
-      const float2 scales = *reinterpret_cast<const float2*>(ring + slot_out * C::SLOT + 2 * kChunk * D);
+      const uint32_t base = ring_addr + slot_out * C::SLOT;
+      const uint8_t* here = ring + slot_out * C::SLOT;
       slot_out = slot_out + 1 == C::STAGES ? 0 : slot_out + 1;
-      if (scales.y == 0.f) { __syncwarp(); continue; }        // a page that holds nothing
-      const int key0 = (s.first_chunk + c) * kChunk;
-      const bool whole = key0 + kChunk <= all_to && key0 >= all_from;
-      const float lv = log2f(scales.y), iv = 1.f / scales.y;
-
-      uint32_t kf[D / 32][4];
+      const int key0 = (s.first_chunk + c) * KEYS;
+      const bool whole = key0 + KEYS <= all_to && key0 >= all_from;
+      float ks[T], lv[T], iv[T];   // a page that holds nothing: log2 0 = -inf hides its keys
 #pragma unroll
-      for (int w = 0; w < D / 32; ++w)
-        ldmatrix_x4(kf[w], kbase + tile_offset<D>((lane & 7) + ((lane >> 3) & 1) * 8, 2 * w + (lane >> 4)));
-      uint32_t pb[NG][2];
+      for (int h = 0; h < T; ++h) {
+        const float2 scales = *reinterpret_cast<const float2*>(here + h * C::TILE + 32 * D);
+        const bool empty = scales.y == 0.f;
+        ks[h] = empty ? 0.f : scales.x;
+        lv[h] = lg2_approx(scales.y);
+        iv[h] = empty ? 0.f : rcp_approx(scales.y);
+      }
+
+      uint32_t kf[T][D / 32][4];
+#pragma unroll
+      for (int h = 0; h < T; ++h)
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w) ldmatrix_x4(kf[h][w], base + h * C::TILE + tile_offset<D>(m_row, 2 * w + m_piece));
+      uint32_t pb[NG][T][2];
 #pragma unroll
       for (int ng = 0; ng < NG; ++ng) {
-        // ---- S^T = K . Q^T: keys g, g + 8, rows 2t, 2t + 1 ----
-        int hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+        // ---- S^T = K . Q^T: keys g, g + 8 of a tile, rows 2t, 2t + 1 ----
+        float x[T][4];
 #pragma unroll
-        for (int w = 0; w < D / 32; ++w) {
-          const uint4 q4 = qf[((rw * NG + ng) * (D / 32) + w) * 32 + lane];
-          mma_s8_16832(hi, kf[w], q4.x, q4.y);
-          mma_s8_16832(lo, kf[w], q4.z, q4.w);
+        for (int h = 0; h < T; ++h) {
+          int hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int w = 0; w < D / 32; ++w) {
+            uint4 q4;
+            if constexpr (C::Q_REGS) q4 = qr[ng][w];
+            else q4 = my_q[(ng * (D / 32) + w) * 32];
+            mma_s8_16832(hi, kf[h][w], q4.x, q4.y);
+            mma_s8_16832(lo, kf[h][w], q4.z, q4.w);
+          }
+          const float f0 = row_scale[ng][0] * ks[h], f1 = row_scale[ng][1] * ks[h];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[h][e] = fmaf((float)(hi[e] * 128 + lo[e]), e & 1 ? f1 : f0, lv[h]);
         }
-        float x[4], mx[2];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = fmaf((float)(hi[e] * 128 + lo[e]), row_scale[ng][e & 1] * scales.x, lv);
         if (!whole) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int i = (r_first + ng * 8 + 2 * t + (e & 1)) / a.G, place = s.place + i, key = key0 + g + 8 * (e >> 1);
-            const bool seen = key < s.len && (!a.causal || key <= place) && (a.window < 0 || key > place - a.window);
-            if (!seen) x[e] = -INFINITY;
+          for (int e = 0; e < 2; ++e) {
+            const int place = s.place + (r_first + ng * 8 + 2 * t + e) / a.G;
+            const int to = a.causal ? min(s.len, place + 1) : s.len, from = a.window >= 0 ? place - a.window + 1 : 0;
+#pragma unroll
+            for (int h = 0; h < T; ++h)
+#pragma unroll
+              for (int k8 = 0; k8 < 2; ++k8) {
+                const int key = key0 + 16 * h + 8 * k8 + g;
+                if (key >= to || key < from) x[h][2 * k8 + e] = -INFINITY;
+              }
           }
         }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          mx[e] = fmaxf(x[e], x[e + 2]);
-          mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 4));
-          mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 8));
-          mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 16));
+        // ---- reference, weights, row sums ----
+        float mx[2] = {fmaxf(x[0][0], x[0][2]), fmaxf(x[0][1], x[0][3])};
+        if constexpr (T == 2) {
+          mx[0] = max3f(mx[0], x[1][0], x[1][2]);
+          mx[1] = max3f(mx[1], x[1][1], x[1][3]);
         }
-        const bool grown = mx[0] > m_run[ng][0] || mx[1] > m_run[ng][1];
-        if (__any_sync(0xffffffffu, grown)) {
+        if (__any_sync(0xffffffffu, mx[0] > m_run[ng][0] + kSlack || mx[1] > m_run[ng][1] + kSlack)) {
           float f[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
+            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 4));
+            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 8));
+            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 16));
             const float m = fmaxf(m_run[ng][e], mx[e]);
             f[e] = ex2_approx(m_run[ng][e] - m);
             m_run[ng][e] = m;
@@ -396,11 +459,14 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
           }
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = ex2_approx(x[e] - m_run[ng][e & 1]);
-        l_run[ng][0] = fmaf(x[0] + x[2], iv, l_run[ng][0]);
-        l_run[ng][1] = fmaf(x[1] + x[3], iv, l_run[ng][1]);
-        pb[ng][0] = transpose8x8(pack2<__half>(x[0], x[1]));
-        pb[ng][1] = transpose8x8(pack2<__half>(x[2], x[3]));
+        for (int h = 0; h < T; ++h) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[h][e] = ex2_approx(x[h][e] - m_run[ng][e & 1]);
+          l_run[ng][0] = fmaf(x[h][0] + x[h][2], iv[h], l_run[ng][0]);
+          l_run[ng][1] = fmaf(x[h][1] + x[h][3], iv[h], l_run[ng][1]);
+          pb[ng][h][0] = transpose8x8(pack2<__half>(x[h][0], x[h][1]));
+          pb[ng][h][1] = transpose8x8(pack2<__half>(x[h][2], x[h][3]));
+        }
       }
       // ---- O^T += V^T . P^T.  A transposing ldmatrix hands out byte pairs of two neighbouring channels for
       // keys 2t, 2t + 1; widened exactly ((b ^ 0x80) | 0x6400 is 1152 + b), channel 2g feeds row g of the
@@ -412,17 +478,19 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
         return *reinterpret_cast<const uint32_t*>(&h);
       };
 #pragma unroll
-      for (int w = 0; w < D / 32; ++w) {
-        uint32_t r[4];
-        ldmatrix_x4_trans(r, vbase + tile_offset<D>((lane & 7) + ((lane >> 3) & 1) * 8, 2 * w + (lane >> 4)));
+      for (int h = 0; h < T; ++h)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t y0 = r[2 * half] ^ 0x80808080u, y1 = r[2 * half + 1] ^ 0x80808080u;
-          const uint32_t va[4] = {widen(y0, 0x4240u), widen(y0, 0x4341u), widen(y1, 0x4240u), widen(y1, 0x4341u)};
+        for (int w = 0; w < D / 32; ++w) {
+          uint32_t r[4];
+          ldmatrix_x4_trans(r, base + h * C::TILE + 16 * D + tile_offset<D>(m_row, 2 * w + m_piece));
 #pragma unroll
-          for (int ng = 0; ng < NG; ++ng) mma_f16_16816(o[ng][2 * w + half], va, pb[ng][0], pb[ng][1]);
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t y0 = r[2 * half] ^ 0x80808080u, y1 = r[2 * half + 1] ^ 0x80808080u;
+            const uint32_t va[4] = {widen(y0, 0x4240u), widen(y0, 0x4341u), widen(y1, 0x4240u), widen(y1, 0x4341u)};
+#pragma unroll
+            for (int ng = 0; ng < NG; ++ng) mma_f16_16816(o[ng][2 * w + half], va, pb[ng][h][0], pb[ng][h][1]);
+          }
         }
-      }
       __syncwarp();
     }
 
@@ -440,50 +508,55 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
     __syncthreads();
     const bool complete = c_begin == 0 && cur.cend == s.chunks;
     const int64_t part = (2ll * blockIdx.x + (c_begin == 0)) * a.rows_per_unit;
+    const float2* my_ml = ml + rw * key_warps * NG * 8;
 #pragma unroll
     for (int ng = 0; ng < NG; ++ng) {
       float f[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float m = kNegSentinel;
-        for (int w = 0; w < key_warps; ++w) m = fmaxf(m, ml[(rw * key_warps + w) * NG * 8 + ng * 8 + 2 * t + e].x);
+        for (int w = 0; w < key_warps; ++w) m = fmaxf(m, my_ml[w * NG * 8 + ng * 8 + 2 * t + e].x);
         f[e] = ex2_approx(m_run[ng][e] - m);
       }
 #pragma unroll
-      for (int d = 0; d < D / 16; ++d) {
-        float* dst = buf + (warp * 8 + 2 * t) * C::BUF_ROW + 16 * d + 2 * g;
-        *reinterpret_cast<float2*>(dst) = make_float2(o[ng][d][0] * f[0], o[ng][d][2] * f[0]);
-        *reinterpret_cast<float2*>(dst + C::BUF_ROW) = make_float2(o[ng][d][1] * f[1], o[ng][d][3] * f[1]);
-      }
-      __syncthreads();
-      for (int idx = kw * 32 + lane; idx < 2 * D; idx += key_warps * 32) {
-        const int row = idx / (D / 4), d4 = idx % (D / 4);
-        float m = kNegSentinel, l = 0.f;
-        for (int w = 0; w < key_warps; ++w) m = fmaxf(m, ml[(rw * key_warps + w) * NG * 8 + ng * 8 + row].x);
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int w = 0; w < key_warps; ++w) {
-          const float2 one = ml[(rw * key_warps + w) * NG * 8 + ng * 8 + row];
-          l += one.y * ex2_approx(one.x - m);
-          const float4 x = *reinterpret_cast<const float4*>(buf + ((rw * key_warps + w) * 8 + row) * C::BUF_ROW + 4 * d4);
-          sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
+      for (int d0 = 0; d0 < D; d0 += C::JOIN) {
+#pragma unroll
+        for (int d = 0; d < C::JOIN / 16; ++d) {
+          float* dst = buf + (warp * 8 + 2 * t) * C::BUF_ROW + 16 * d + 2 * g;
+          const float* x = o[ng][d0 / 16 + d];
+          *reinterpret_cast<float2*>(dst) = make_float2(x[0] * f[0], x[2] * f[0]);
+          *reinterpret_cast<float2*>(dst + C::BUF_ROW) = make_float2(x[1] * f[1], x[3] * f[1]);
         }
-        const int r_local = (rw * NG + ng) * 8 + row, r = row0 + r_local;
-        if (complete) {
-          if (r < a.rows) {
-            const int i = r / a.G, head = hkv * a.G + r % a.G;
-            const float inv = (i < s.n && l != 0.f) ? 1.f / l : 0.f;
-            if (inv == 0.f) sum = make_float4(0.f, 0.f, 0.f, 0.f);
-            uint2 y;
-            if (a.bf16) y = make_uint2(pack2<__nv_bfloat16>(sum.x * inv, sum.y * inv), pack2<__nv_bfloat16>(sum.z * inv, sum.w * inv));
-            else y = make_uint2(pack2<__half>(sum.x * inv, sum.y * inv), pack2<__half>(sum.z * inv, sum.w * inv));
-            *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + cur.b * a.o_sb + head * a.o_sh + i * a.o_ss + 4 * d4) = y;
+        __syncthreads();
+        for (int idx = kw * 32 + lane; idx < 2 * C::JOIN; idx += key_warps * 32) {
+          const int row = idx / (C::JOIN / 4), ch = idx % (C::JOIN / 4) * 4;
+          float m = kNegSentinel, l = 0.f;
+          for (int w = 0; w < key_warps; ++w) m = fmaxf(m, my_ml[w * NG * 8 + ng * 8 + row].x);
+          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int w = 0; w < key_warps; ++w) {
+            const float2 one = my_ml[w * NG * 8 + ng * 8 + row];
+            l = fmaf(one.y, ex2_approx(one.x - m), l);
+            const float4 x = *reinterpret_cast<const float4*>(buf + ((rw * key_warps + w) * 8 + row) * C::BUF_ROW + ch);
+            sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
           }
-        } else {
-          *reinterpret_cast<float4*>(a.part_o + (part + r_local) * D + 4 * d4) = sum;
-          if (d4 == 0) *reinterpret_cast<float2*>(a.part_ml + (part + r_local) * 2) = make_float2(m, l);
+          const int r_local = (rw * NG + ng) * 8 + row, r = row0 + r_local;
+          if (complete) {
+            if (r < a.rows) {
+              const int i = r / a.G, head = hkv * a.G + r % a.G;
+              const float inv = (i < s.n && l != 0.f) ? 1.f / l : 0.f;
+              if (inv == 0.f) sum = make_float4(0.f, 0.f, 0.f, 0.f);
+              uint2 y;
+              if (a.bf16) y = make_uint2(pack2<__nv_bfloat16>(sum.x * inv, sum.y * inv), pack2<__nv_bfloat16>(sum.z * inv, sum.w * inv));
+              else y = make_uint2(pack2<__half>(sum.x * inv, sum.y * inv), pack2<__half>(sum.z * inv, sum.w * inv));
+              *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + cur.b * a.o_sb + head * a.o_sh + i * a.o_ss + d0 + ch) = y;
+            }
+          } else {
+            *reinterpret_cast<float4*>(a.part_o + (part + r_local) * D + d0 + ch) = sum;
+            if (d0 + ch == 0) *reinterpret_cast<float2*>(a.part_ml + (part + r_local) * 2) = make_float2(m, l);
+          }
         }
+        __syncthreads();
       }
-      __syncthreads();
     }
     if (cur.left <= 0) break;
     next_unit(cur);
@@ -496,15 +569,22 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
 // without keys or queries.  One block per unit, one warp per row at a time.
 template <int D>
 __global__ void __launch_bounds__(kPaThreads) paged_join_kernel(const PagedArgs a) {
-  __shared__ long long red[kPaWarps][2];
+  __shared__ unsigned red[kPaWarps];
+  __shared__ unsigned s_before;
   const int units = a.Hkv * a.row_units;
   const int b = blockIdx.x / units, u = blockIdx.x - b * units;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Line line = line_of(a, b, units, red);
+  const Line line = line_of(a, units, red);
+  if (line.b0 <= b && b < line.b1) {               // the chunks of the sequences before b
+    unsigned at = line.begin;
+    for (int j = line.b0; j < b; ++j) at += seq_of(a, j).chunks * units;
+    s_before = at;
+  }
+  __syncthreads();
   const Seq s = seq_of(a, b);
-  const long long per = share_of(line.total, a.blocks);
-  const long long g0 = line.before + (long long)u * s.chunks;
-  const long long i0 = g0 / per, i1 = s.chunks > 0 ? (g0 + s.chunks - 1) / per : i0;
+  const unsigned per = share_of(line.total, a.blocks);
+  const unsigned g0 = s_before + (unsigned)u * s.chunks;
+  const unsigned i0 = g0 / per, i1 = s.chunks > 0 ? (g0 + s.chunks - 1) / per : i0;
   // every block waits, also one with nothing to do: a grid that ended before the split kernel would let
   // the stream's next kernel start beside it
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -521,7 +601,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_join_kernel(const PagedArgs 
       // partial n: block i0 + n, its slot 1 where it began the unit (n = 0), else slot 0
       float m = kNegSentinel;
       const int parts = (int)(i1 - i0 + 1);
-      auto row_of = [&](int n) { return (2 * (i0 + n) + (n == 0)) * a.rows_per_unit + r_local; };
+      auto row_of = [&](int n) { return (int64_t)(2 * (i0 + n) + (n == 0)) * a.rows_per_unit + r_local; };
       for (int n = lane; n < parts; n += 32) m = fmaxf(m, a.part_ml[row_of(n) * 2]);
 #pragma unroll
       for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -560,16 +640,14 @@ struct Plan {
 Plan plan_of(const sl8_paged_cache& c, const sl8_paged_attn_params& p) {
   Plan x{};
   const int64_t rows = (int64_t)p.M * (p.Hq / c.Hkv);
-  const int most = c.D == 256 ? 2 : 4;            // accumulators: D / 4 * NG registers a thread
-  x.ng = rows <= 8 ? 1 : (rows <= 16 ? 2 : most);
-  x.row_warps = 1;
-  const int groups = c.D == 256 ? 4 : 8;          // PaCfg::GROUPS
-  while (x.row_warps * x.ng * 8 < rows && x.row_warps * x.ng < groups) x.row_warps *= 2;
+  x.ng = rows <= 8 ? 1 : (rows <= 16 ? 2 : groups_of(c.D));
+  x.row_warps = rows > 8 * groups_of(c.D) ? 2 : 1;   // PaCfg::ROW_WARPS
   x.rows_per_unit = x.row_warps * x.ng * 8;
   x.row_units = (int)((rows + x.rows_per_unit - 1) / x.rows_per_unit);
   const int64_t held = (int64_t)c.max_pages * c.page_size;
   const int64_t longest = p.max_context_len > 0 && p.max_context_len < held ? p.max_context_len : held;
-  const int64_t chunks = (longest + kChunk - 1) / kChunk * p.B * c.Hkv * x.row_units;
+  const int keys = 1 << chunk_shift_of(c.D, x.ng);
+  const int64_t chunks = (longest + keys - 1) / keys * p.B * c.Hkv * x.row_units;
   const int64_t want = (chunks + kPaWarps - 1) / kPaWarps;
   x.blocks = (int)(want < 1 ? 1 : (want > kNumSms ? kNumSms : want));
   return x;
@@ -592,7 +670,7 @@ int launch_paged(const PagedArgs& a, cudaStream_t stream) {
   SL8_CUDA_TRY(cudaGetDevice(&dev));
   if (dev >= 64 || !allowed[dev].load()) {
     SL8_CUDA_TRY(cudaFuncSetAttribute(paged_split_kernel<D, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      PaCfg<D, NG>::smem(PaCfg<D, NG>::GROUPS / NG)));
+                                      PaCfg<D, NG>::smem(PaCfg<D, NG>::ROW_WARPS)));
     if (dev < 64) allowed[dev].store(true);
   }
   const int smem = PaCfg<D, NG>::smem(a.row_warps);
@@ -647,7 +725,9 @@ extern "C" int sl8_attn_paged(const sl8_paged_cache* c, const sl8_paged_attn_par
   if (workspace == nullptr || workspace_bytes < sl8_attn_paged_workspace(c, p)) return SL8_ERR_WORKSPACE;
   if (!aligned16(workspace)) return SL8_ERR_MISALIGNED;
   const Plan x = plan_of(*c, *p);
-  if ((int64_t)p->B * c->Hkv * x.row_units > 0x7fffffffll) return SL8_ERR_TOO_LARGE;
+  // the line of all chunks is counted in 32 bits; its length is bounded by what the table can name
+  const int64_t most = ((int64_t)c->max_pages * c->page_size + 31) / 16 * p->B * c->Hkv * x.row_units;
+  if ((int64_t)p->B * c->Hkv * x.row_units > 0x7fffffffll || most > 0x7fffffffll) return SL8_ERR_TOO_LARGE;
   PagedArgs a{};
   a.q = p->q; a.q_sb = p->q_stride_b; a.q_sh = p->q_stride_h; a.q_ss = p->q_stride_s;
   a.out = p->out; a.o_sb = p->out_stride_b; a.o_sh = p->out_stride_h; a.o_ss = p->out_stride_s;
@@ -659,6 +739,7 @@ extern "C" int sl8_attn_paged(const sl8_paged_cache* c, const sl8_paged_attn_par
   a.page_shift = page_shift_of(c->page_size); a.num_pages = c->num_pages; a.max_pages = held ? c->max_pages : 0;
   a.causal = p->causal; a.window = p->window_left; a.bf16 = p->dtype == SL8_BF16;
   a.row_warps = x.row_warps; a.rows_per_unit = x.rows_per_unit; a.row_units = x.row_units; a.blocks = x.blocks;
+  a.chunk_shift = chunk_shift_of(c->D, x.ng);
   a.scale_log2 = p->softmax_scale * 1.4426950408889634f;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (c->D) {
