@@ -102,9 +102,11 @@ int sl8_kv_read_paged(const sl8_paged_cache* cache, int32_t B, const int32_t* fi
  * sequence b is the token at place context_lens[b] - query_lens[b] + i (query_lens NULL: M); rows past
  * query_lens[b] give zeros, so does a row that sees no key.  causal != 0: it sees the keys up to its own
  * place, else all of the context; window_left >= 0: only keys in (place - window_left, ...].
- * max_context_len (host): an upper bound of context_lens that sizes the launch; <= 0 = max_pages *
- * page_size.  Longer sequences are still computed in full.
- * workspace: sl8_attn_paged_workspace() bytes, any contents; a workspace serves one call at a time.
+ * max_context_len (host): an upper bound of context_lens that sizes the launch and the workspace (keys at or
+ * past it are not seen); <= 0 = max_pages * page_size.
+ * Two kernels: a split one that streams the pages (rows M * Hq / Hkv up to 64: decode, drafted tokens), and a
+ * tensor-memory one over a dense copy of the codes in the workspace (more rows; D 64 / 128 / 256, scale >= 0).
+ * workspace: sl8_attn_paged_workspace() bytes, 16-byte aligned, any contents; it serves one call at a time.
  */
 typedef struct sl8_paged_attn_params {
   const void* q; void* out;
@@ -117,6 +119,10 @@ typedef struct sl8_paged_attn_params {
 size_t sl8_attn_paged_workspace(const sl8_paged_cache* cache, const sl8_paged_attn_params* p);
 int sl8_attn_paged(const sl8_paged_cache* cache, const sl8_paged_attn_params* p, void* workspace,
                    size_t workspace_bytes, void* stream);
+
+/* Synchronises the stream and returns the status of the tensor-memory kernel's bounded waits on the current
+ * device since the last call (SL8_OK or SL8_ERR_DEVICE_TIMEOUT), and clears it. */
+int sl8_paged_status(void* stream);
 
 #ifdef __cplusplus
 }

@@ -90,6 +90,9 @@ def device_status(device=None) -> int:
         rc = lib.sl8_read_device_status(_ptr(bws), _stream(device))
     if rc == 0 and _ext is not None:
         rc = int(_ext.device_status(torch.empty(0, device=device)))
+    if rc == 0:
+        with torch.cuda.device(device):
+            rc = lib.sl8_paged_status(_stream(device))
     return rc
 
 

@@ -208,6 +208,7 @@ SIGNATURES = {
                                     C.c_void_p]),
     "sl8_attn_paged_workspace": (C.c_size_t, [C.POINTER(PagedCache), C.POINTER(PagedAttnParams)]),
     "sl8_attn_paged": (C.c_int, [C.POINTER(PagedCache), C.POINTER(PagedAttnParams), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "sl8_paged_status": (C.c_int, [C.c_void_p]),
     "sl8_tensor_peak_probe": (C.c_int, [C.c_int, C.c_int, C.POINTER(C.c_double), C.c_void_p, C.c_size_t, C.c_void_p]),
     "sl8_tensor_peak_probe_n": (C.c_int, [C.c_int, C.c_int, C.c_int, C.POINTER(C.c_double), C.c_void_p, C.c_size_t, C.c_void_p]),
     "sl8_decode_static_status": (C.c_int, [C.c_void_p]),

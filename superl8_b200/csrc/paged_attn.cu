@@ -19,7 +19,7 @@
 // of a one-block-per-SM grid, whatever the lengths are; a unit that lies in one range is finished there,
 // the others leave (O, M, l) partials that a second kernel joins.  The loads run ahead across unit
 // boundaries, so merging a unit's warps does not drain the ring.
-#include "sl8_common.cuh"
+#include "sl8_paged.cuh"
 #include "sl8_mma.cuh"
 
 #include <atomic>
@@ -29,49 +29,6 @@ namespace {
 
 constexpr int kPaWarps = 8;
 constexpr int kPaThreads = 32 * kPaWarps;
-
-struct PagedArgs {
-  const void* q;
-  int64_t q_sb, q_sh, q_ss;
-  void* out;
-  int64_t o_sb, o_sh, o_ss;
-  const int8_t *k, *v;
-  const float *ks, *vs;
-  const int32_t* table;
-  int64_t table_stride;
-  const int32_t* lens;
-  const int32_t* query_lens;
-  float* part_o;      // [2 * blocks][rows_per_unit][D]
-  float* part_ml;     // [2 * blocks][rows_per_unit][2]
-  int B, Hq, Hkv, M, G, rows;              // rows = M * G query rows per (sequence, KV head)
-  int page_shift, num_pages, max_pages;
-  int causal, window, bf16;
-  int row_warps;      // warps that share a key but hold other rows (1 or 2)
-  int rows_per_unit, row_units;            // rows = up to row_units * rows_per_unit
-  int blocks;         // blocks of the split kernel
-  int chunk_shift;    // log2 of the keys per warp and step
-  float scale_log2;   // softmax_scale * log2 e
-};
-
-// What a sequence asks for: tokens that exist, its query tokens, the first chunk a query can see.
-struct Seq {
-  int len, n, first_chunk, chunks;
-  int place;   // of query token 0
-};
-
-__device__ __forceinline__ Seq seq_of(const PagedArgs& a, int b) {
-  Seq s;
-  const int context = __ldg(a.lens + b);
-  s.n = a.query_lens ? min(max(__ldg(a.query_lens + b), 0), a.M) : a.M;
-  const int64_t held = (int64_t)a.max_pages << a.page_shift;
-  s.len = (int)min((int64_t)max(context, 0), held);
-  s.place = max(context, 0) - s.n;
-  int64_t lo = 0;
-  if (a.window >= 0) lo = max((int64_t)0, (int64_t)s.place - a.window + 1);
-  s.first_chunk = (int)(lo >> a.chunk_shift);
-  s.chunks = (s.n > 0 && lo < s.len) ? (int)(((int64_t)s.len + (1 << a.chunk_shift) - 1) >> a.chunk_shift) - s.first_chunk : 0;
-  return s;
-}
 
 // The line: the chunks of all units, sequence by sequence (the host bounds it below 2^31).  Every thread owns
 // a run of ceil(B / threads) sequences; returns the line's length and the place where the run begins.
@@ -626,30 +583,49 @@ __global__ void __launch_bounds__(kPaThreads) paged_join_kernel(const PagedArgs 
   }
 }
 
+// Rows that one unit of the split kernel serves: 8 per group of the MMA's N axis, groups per warp (NG), warps
+// with other rows.
+struct Plan {
+  int ng, row_warps, row_units, rows_per_unit, blocks;
+  size_t prefill_bytes;   // > 0: paged_prefill.cu serves the call, with this workspace
+};
+
+// Rows per (sequence, KV head) from which the tensor-memory kernel serves a call.
+constexpr int kPrefillRows = 65;
+
 int page_shift_of(int page_size) {
   for (int s = 4; s <= 8; ++s)
     if (page_size == (1 << s)) return s;
   return -1;
 }
 
-// Rows that one unit serves: 8 per group of the MMA's N axis, groups per warp (NG), warps with other rows.
-struct Plan {
-  int ng, row_warps, row_units, rows_per_unit, blocks;
-};
+PagedArgs args_of(const sl8_paged_cache& c, const sl8_paged_attn_params& p) {
+  PagedArgs a{};
+  a.q = p.q; a.q_sb = p.q_stride_b; a.q_sh = p.q_stride_h; a.q_ss = p.q_stride_s;
+  a.out = p.out; a.o_sb = p.out_stride_b; a.o_sh = p.out_stride_h; a.o_ss = p.out_stride_s;
+  a.k = c.k; a.v = c.v; a.ks = c.k_scale; a.vs = c.v_scale;
+  a.table = c.block_table; a.table_stride = c.table_stride; a.lens = c.context_lens; a.query_lens = p.query_lens;
+  a.B = p.B; a.Hq = p.Hq; a.Hkv = c.Hkv; a.M = p.M; a.G = p.Hq / c.Hkv; a.rows = p.M * a.G;
+  a.page_shift = page_shift_of(c.page_size); a.num_pages = c.num_pages;
+  int64_t tokens = c.num_pages > 0 ? (int64_t)c.max_pages * c.page_size : 0;
+  if (p.max_context_len > 0 && p.max_context_len < tokens) tokens = p.max_context_len;
+  a.max_tokens = (int)(tokens < 0x7fffffff ? tokens : 0x7fffffff);
+  a.causal = p.causal; a.window = p.window_left; a.bf16 = p.dtype == SL8_BF16;
+  a.scale_log2 = p.softmax_scale * 1.4426950408889634f;
+  return a;
+}
 
-Plan plan_of(const sl8_paged_cache& c, const sl8_paged_attn_params& p) {
+Plan plan_of(const PagedArgs& a, int D) {
   Plan x{};
-  const int64_t rows = (int64_t)p.M * (p.Hq / c.Hkv);
-  x.ng = rows <= 8 ? 1 : (rows <= 16 ? 2 : groups_of(c.D));
-  x.row_warps = rows > 8 * groups_of(c.D) ? 2 : 1;   // PaCfg::ROW_WARPS
+  x.ng = a.rows <= 8 ? 1 : (a.rows <= 16 ? 2 : groups_of(D));
+  x.row_warps = a.rows > 8 * groups_of(D) ? 2 : 1;   // PaCfg::ROW_WARPS
   x.rows_per_unit = x.row_warps * x.ng * 8;
-  x.row_units = (int)((rows + x.rows_per_unit - 1) / x.rows_per_unit);
-  const int64_t held = (int64_t)c.max_pages * c.page_size;
-  const int64_t longest = p.max_context_len > 0 && p.max_context_len < held ? p.max_context_len : held;
-  const int keys = 1 << chunk_shift_of(c.D, x.ng);
-  const int64_t chunks = (longest + keys - 1) / keys * p.B * c.Hkv * x.row_units;
+  x.row_units = (a.rows + x.rows_per_unit - 1) / x.rows_per_unit;
+  const int keys = 1 << chunk_shift_of(D, x.ng);
+  const int64_t chunks = ((int64_t)a.max_tokens + keys - 1) / keys * a.B * a.Hkv * x.row_units;
   const int64_t want = (chunks + kPaWarps - 1) / kPaWarps;
   x.blocks = (int)(want < 1 ? 1 : (want > kNumSms ? kNumSms : want));
+  x.prefill_bytes = a.rows >= kPrefillRows ? sl8_paged_prefill_workspace(a, D) : 0;
   return x;
 }
 
@@ -706,9 +682,10 @@ int launch_paged_rows(const PagedArgs& a, int ng, cudaStream_t stream) {
 using namespace sl8;
 
 extern "C" size_t sl8_attn_paged_workspace(const sl8_paged_cache* c, const sl8_paged_attn_params* p) {
-  if (paged_checks(c, p) != SL8_OK || (int64_t)p->B * p->Hq * p->M == 0) return 256;
-  const Plan x = plan_of(*c, *p);
-  return 256 + (size_t)2 * x.blocks * x.rows_per_unit * (c->D + 2) * sizeof(float);
+  if (paged_checks(c, p) != SL8_OK || (int64_t)p->B * p->Hq * p->M == 0) return 1024;
+  const Plan x = plan_of(args_of(*c, *p), c->D);
+  if (x.prefill_bytes > 0) return 1024 + x.prefill_bytes;
+  return 1024 + (size_t)2 * x.blocks * x.rows_per_unit * (c->D + 2) * sizeof(float);
 }
 
 extern "C" int sl8_attn_paged(const sl8_paged_cache* c, const sl8_paged_attn_params* p, void* workspace, size_t workspace_bytes,
@@ -722,26 +699,21 @@ extern "C" int sl8_attn_paged(const sl8_paged_cache* c, const sl8_paged_attn_par
   if (!aligned16(p->q) || !aligned16(p->out) || (held && (!aligned16(c->k) || !aligned16(c->v)))) return SL8_ERR_MISALIGNED;
   if (p->q_stride_b % 8 || p->q_stride_h % 8 || p->q_stride_s % 8 || p->out_stride_b % 8 || p->out_stride_h % 8 || p->out_stride_s % 8)
     return SL8_ERR_MISALIGNED;
+  if ((int64_t)p->M * (p->Hq / c->Hkv) > 0x7fffffffll - 128) return SL8_ERR_TOO_LARGE;
   if (workspace == nullptr || workspace_bytes < sl8_attn_paged_workspace(c, p)) return SL8_ERR_WORKSPACE;
   if (!aligned16(workspace)) return SL8_ERR_MISALIGNED;
-  const Plan x = plan_of(*c, *p);
-  // the line of all chunks is counted in 32 bits; its length is bounded by what the table can name
-  const int64_t most = ((int64_t)c->max_pages * c->page_size + 31) / 16 * p->B * c->Hkv * x.row_units;
-  if ((int64_t)p->B * c->Hkv * x.row_units > 0x7fffffffll || most > 0x7fffffffll) return SL8_ERR_TOO_LARGE;
-  PagedArgs a{};
-  a.q = p->q; a.q_sb = p->q_stride_b; a.q_sh = p->q_stride_h; a.q_ss = p->q_stride_s;
-  a.out = p->out; a.o_sb = p->out_stride_b; a.o_sh = p->out_stride_h; a.o_ss = p->out_stride_s;
-  a.k = c->k; a.v = c->v; a.ks = c->k_scale; a.vs = c->v_scale;
-  a.table = c->block_table; a.table_stride = c->table_stride; a.lens = c->context_lens; a.query_lens = p->query_lens;
-  a.part_o = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + 256);
-  a.part_ml = a.part_o + (size_t)2 * x.blocks * x.rows_per_unit * c->D;
-  a.B = p->B; a.Hq = p->Hq; a.Hkv = c->Hkv; a.M = p->M; a.G = p->Hq / c->Hkv; a.rows = p->M * a.G;
-  a.page_shift = page_shift_of(c->page_size); a.num_pages = c->num_pages; a.max_pages = held ? c->max_pages : 0;
-  a.causal = p->causal; a.window = p->window_left; a.bf16 = p->dtype == SL8_BF16;
-  a.row_warps = x.row_warps; a.rows_per_unit = x.rows_per_unit; a.row_units = x.row_units; a.blocks = x.blocks;
-  a.chunk_shift = chunk_shift_of(c->D, x.ng);
-  a.scale_log2 = p->softmax_scale * 1.4426950408889634f;
+  PagedArgs a = args_of(*c, *p);
+  const Plan x = plan_of(a, c->D);
+  uint8_t* ws = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 1023) & ~uintptr_t(1023));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  a.chunk_shift = chunk_shift_of(c->D, x.ng);
+  if (x.prefill_bytes > 0) return sl8_paged_prefill(a, c->D, ws, x.prefill_bytes, s);
+  // the line of all chunks is counted in 32 bits; its length is bounded by what can be seen
+  const int64_t most = ((int64_t)a.max_tokens + 31) / 16 * p->B * c->Hkv * x.row_units;
+  if ((int64_t)p->B * c->Hkv * x.row_units > 0x7fffffffll || most > 0x7fffffffll) return SL8_ERR_TOO_LARGE;
+  a.part_o = reinterpret_cast<float*>(ws);
+  a.part_ml = a.part_o + (size_t)2 * x.blocks * x.rows_per_unit * c->D;
+  a.row_warps = x.row_warps; a.rows_per_unit = x.rows_per_unit; a.row_units = x.row_units; a.blocks = x.blocks;
   switch (c->D) {
     case 32: return launch_paged_rows<32>(a, x.ng, s);
     case 64: return launch_paged_rows<64>(a, x.ng, s);

@@ -74,7 +74,9 @@ def attn_paged_cached(q, k_i8, k_scale, v_i8, v_scale, block_table, context_lens
     sequence b is the token at place ``context_lens[b] - query_lens[b] + i`` (``query_lens`` int32 [B],
     None: M for all; rows past it give zeros) and sees the keys up to its own place, or all of the context
     with ``causal=False``; ``window_left`` >= 0 leaves only keys in (place - window_left, ...].  A row that
-    sees no key gives zeros.  ``max_context_len`` (host) is an upper bound of ``context_lens`` that sizes
-    the launch; None takes what the table can hold."""
+    sees no key gives zeros.  ``max_context_len`` (host) is an upper bound of ``context_lens`` (keys at
+    or past it are not seen); None takes what the table can hold.  With more than 64 query rows per KV
+    head (M H_q / H_kv) the call widens the codes into a workspace of 4 D bytes per key and KV head,
+    at most 192 MiB or one (sequence, head) at a time, sized by that bound."""
     return _C.attn_paged(q, k_i8, k_scale, v_i8, v_scale, block_table, context_lens, scale, causal, window_left, query_lens,
                          max_context_len)

@@ -64,20 +64,24 @@ def dequant(codes, scale, table, n, first=0):
     return out, there
 
 
-def attend(q, k_i8, k_scale, v_i8, v_scale, table, lens, scale=None, causal=True, window=-1, query_lens=None):
-    """(out, tolerance) fp64 [B, Hq, M, D]; the tolerance bounds a kernel that splits q into two int8 planes,
-    rounds the weights to fp16 against their maximum, sums in fp32 and rounds once at the end."""
+def attend(q, k_i8, k_scale, v_i8, v_scale, table, lens, scale=None, causal=True, window=-1, query_lens=None,
+           limit=None):
+    """(out, tolerance) fp64 [B, Hq, M, D]; the tolerance bounds a kernel that splits q into two int8 planes (or
+    takes it as it is), rounds the weights to q's 16-bit type (or fp16) against their maximum, sums in fp32 and
+    rounds once at the end.  Keys at or past ``limit`` are not seen."""
     q_dt = q.dtype
     B, Hq, M, D = q.shape
     P, H, page, _ = k_i8.shape
     G = Hq // H
     scale = D ** -0.5 if scale is None else scale
+    # up to 64 rows per KV head the weights are fp16, above (the tensor-memory kernel) they have q's type
+    weight_err = U[q_dt] if M * G > 64 else U[torch.float16]
     out, tol = torch.zeros(B, Hq, M, D, dtype=F64), torch.zeros(B, Hq, M, D, dtype=F64)
     for b in range(B):
         row = table[b].tolist()
         total = max(0, int(lens[b]))
         m = M if query_lens is None else min(M, max(0, int(query_lens[b])))
-        n = min(total, len(row) * page)
+        n = min(total, len(row) * page, total if limit is None else limit)
         if n == 0 or m == 0:
             continue
         K, there = dequant(k_i8, k_scale, row, n)
@@ -106,8 +110,8 @@ def attend(q, k_i8, k_scale, v_i8, v_scale, table, lens, scale=None, causal=True
                 amax = x.abs().amax(1, keepdim=True)
                 size = torch.where(seen, logit.abs(), torch.zeros_like(p)).amax(1, keepdim=True)
                 ell = abs(scale) * amax / 32512 * K[h].abs().sum(1).max() + size * 2.0 ** -21 + 2.0 ** -20
-                # weights: fp16 rounding 2^-11, exponential and sums in fp32 (2^-18 covers a few thousand terms)
-                rel = torch.expm1(2 * ell) + 2.0 ** -11 + 2.0 ** -18
+                # weights: their 16-bit rounding, exponential and sums in fp32 (2^-18 covers a few thousand terms)
+                rel = torch.expm1(2 * ell) + weight_err + 2.0 ** -18
                 big = (p * vs[h]).amax(1, keepdim=True)
                 code = torch.where(vs[h] > 0, 1 / vs[h], torch.zeros_like(vs[h])).unsqueeze(1) * V[h].abs()
                 t = rel * (p @ V[h].abs()) + big * 2.0 ** -24 * code.sum(0)

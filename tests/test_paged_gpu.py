@@ -222,8 +222,7 @@ def held_to(out, q, cache, table, lens, **kw):
     assert torch.isfinite(out.float()).all() and (off <= tol).all(), float((off / tol.clamp(min=1e-30)).max())
 
 
-@pytest.mark.parametrize("case", ATTEND)
-def test_attend_against_definition(device, binding, case):
+def attend_case(device, case):
     lens, Hq, Hkv, M, D, page, dtype, causal, window, query_lens = case
     B = len(lens)
     table, pages = po.pages_for(lens, page, seed=sum(lens))
@@ -235,6 +234,11 @@ def test_attend_against_definition(device, binding, case):
                                query_lens=None if ql is None else ql.to(device))
     assert out.shape == q.shape and out.dtype == dtype
     held_to(out, q, cache, table, lens, causal=causal, window=window, query_lens=query_lens)
+
+
+@pytest.mark.parametrize("case", ATTEND)
+def test_attend_against_definition(device, binding, case):
+    attend_case(device, case)
 
 
 def test_attend_scales_of_very_different_pages(device):
@@ -336,14 +340,75 @@ def test_attend_strides_streams_and_repeats(device, binding):
     assert (one.float() - ref[:1].float()).abs().max() <= 4 * 2.0 ** -11 * ref.float().abs().max()
 
 
-def test_attend_understated_length_is_still_whole(device):
-    """max_context_len sizes the launch, it does not cut the context."""
-    lens, page, D = [5000, 3000], 64, 128
+@pytest.mark.parametrize("M", [1, 70])
+def test_attend_sees_no_key_past_the_stated_length(device, M):
+    lens, page, D = [500, 300, 100], 64, 64
     table, pages = po.pages_for(lens, page)
     cache = po.random_cache(pages, 2, page, D)
-    q = torch.randn(2, 4, 1, D, generator=torch.Generator().manual_seed(9)).half()
+    q = torch.randn(3, 4, M, D, generator=torch.Generator().manual_seed(9)).half()
     args = on(device, q, *cache, table, torch.tensor(lens, dtype=torch.int32))
-    held_to(s8.attn_paged_cached(*args, max_context_len=16), q, cache, table, lens)
+    for limit in (500, 333, 16, 1):
+        held_to(s8.attn_paged_cached(*args, max_context_len=limit), q, cache, table, lens, limit=limit)
+
+
+PREFILL = [  # lens, Hq, Hkv, M, D, page, dtype, causal, window, query_lens
+    ([200], 4, 4, 200, 128, 16, torch.float16, True, -1, None),
+    ([300, 77, 0, 129], 8, 2, 77, 128, 64, torch.bfloat16, True, -1, [77, 77, 0, 40]),
+    ([700, 130], 4, 1, 65, 64, 32, torch.float16, True, -1, None),
+    ([260, 64], 28, 4, 33, 128, 128, torch.float16, True, 50, [33, 20]),
+    ([400], 6, 6, 150, 256, 16, torch.bfloat16, True, -1, None),
+    ([190, 70], 4, 2, 128, 64, 256, torch.bfloat16, False, -1, [100, 70]),
+    ([90], 2, 2, 130, 128, 16, torch.float16, True, -1, None),          # more queries than context
+    ([333], 3, 1, 90, 64, 16, torch.float16, False, 100, None),
+    ([150], 2, 1, 70, 128, 16, torch.float16, True, 0, None),
+    ([129], 16, 1, 17, 32, 16, torch.float16, True, -1, None),          # D = 32: the split kernel, several row units
+]
+
+
+@pytest.mark.parametrize("case", PREFILL)
+def test_many_rows_against_definition(device, binding, case):
+    attend_case(device, case)
+    assert _C.device_status() == 0
+
+
+def test_many_rows_missing_pages_scales_and_groups(device):
+    """Missing and empty pages, V scales far apart, a negative softmax scale (the split kernel serves it), rows in
+    a strided layout; and a batch whose dense copies are made in several groups."""
+    lens, page, D, M = [150, 90], 16, 128, 40
+    table, pages = po.pages_for(lens, page, spare=3)
+    cache = list(po.random_cache(pages, 2, page, D, seed=6))
+    table[0, 2], table[0, 4] = -1, pages + 7
+    empty = int(table[1, 1])
+    cache[1][empty] = cache[3][empty] = 0
+    cache[3] = cache[3] * torch.tensor([1e-2, 1.0, 1e2, 3.0, 0.1, 10.0] * 9)[:pages].unsqueeze(1)
+    q = torch.randn(2, M, 8, 2 * D, generator=torch.Generator().manual_seed(7)).half()[..., :D].transpose(1, 2)
+    lens_t = torch.tensor(lens, dtype=torch.int32)
+    for scale in (None, 0.2, -0.05):
+        out = s8.attn_paged_cached(*on(device, q, *cache, table, lens_t), scale=scale)
+        held_to(out, q, cache, table, lens, scale=scale)
+    bad = q.clone()
+    bad[1, 3, 5, 2] = float("nan")
+    out = s8.attn_paged_cached(*on(device, bad, *cache, table, lens_t))
+    assert torch.isnan(out[1, 3, 5].float()).all()
+    out[1, 3, 5] = 0
+    assert torch.isfinite(out.float()).all()
+    # 3 x 8 units of 30016 keys at D = 128 are 369 MB of dense copies: two groups; against one sequence at a time
+    g = torch.Generator(device=device).manual_seed(11)
+    lens = [30000, 29000, 257]
+    table, pages = po.pages_for(lens, 128)
+    big = [torch.randint(-127, 128, (pages, 8, 128, D), dtype=torch.int8, device=device, generator=g) for _ in "kv"]
+    sc = [torch.rand(pages, 8, device=device, generator=g) * 0.02 + 0.01 for _ in "kv"]
+    cache = (big[0], sc[0], big[1], sc[1])
+    q = torch.randn(3, 16, 40, D, device=device, generator=g).half()
+    args = on(device, table, torch.tensor(lens, dtype=torch.int32))
+    out = s8.attn_paged_cached(q, *cache, *args, max_context_len=30000)
+    for b in range(3):
+        one = s8.attn_paged_cached(q[b:b + 1], *cache, args[0][b:b + 1], args[1][b:b + 1], max_context_len=lens[b])
+        assert torch.equal(out[b:b + 1], one)
+    # and the first rows against the split kernel (up to 64 rows: 20 tokens of 2 heads per KV head)
+    few = s8.attn_paged_cached(q[:, :, 20:], *cache, *args, max_context_len=30000)
+    assert (few.float() - out[:, :, 20:].float()).abs().max() <= 0.01 * out.float().abs().max()
+    assert _C.device_status() == 0
 
 
 def test_serving_loop_and_graphs(device):
