@@ -538,7 +538,7 @@ def _rows(t, aligned):
     ok = t.stride(3) == 1 or t.shape[3] == 1
     if aligned and ok:
         ok = t.data_ptr() % 16 == 0 and all(t.shape[d] <= 1 or t.stride(d) % 8 == 0 for d in range(3))
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+    return t if ok else t.detach().clone(memory_format=torch.contiguous_format)
 
 
 def _steps(t, name):

@@ -9,7 +9,7 @@ import math
 
 import torch
 
-from . import _C
+from . import _C, _lib
 from .quant import quantize_qk
 
 
@@ -100,8 +100,8 @@ def attn_ref(q, k, v, *, causal: bool = False, scale: float | None = None):
 
 
 class _Rope(torch.autograd.Function):
-    """The rotation is linear and orthogonal: its gradient is the rotation by the opposite angle, itself
-    differentiable the same way."""
+    """apply_rope's gradient under the ctypes binding (the compiled one has its own): the rotation is linear and
+    orthogonal, so its gradient is the rotation by the opposite angle, itself differentiable the same way."""
 
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, freq_axis, interleaved, inverse):
@@ -134,6 +134,10 @@ def apply_rope(q, k, positions, inv_freq, *, freq_axis=None, interleaved: bool =
     place.  Angles are formed in 64 bits, so far positions keep their precision.  Differentiable in q and
     k (also twice); ``inv_freq`` is a constant.  What it returns is what ``attn``, ``attn_int8_fwd`` and the
     other prefill operators take; ``kv_append_paged`` does the same rotation on the way into a cache."""
+    if _C._compiled():
+        r = _C._ext.apply_rope(q, k, positions, inv_freq, freq_axis, bool(interleaved))
+        _lib.launches += 1 if (r[0].numel() or (k is not None and k.numel())) else 0
+        return r
     if inv_freq.requires_grad:
         raise RuntimeError("superl8_b200 apply_rope: inv_freq is a constant (no gradient is computed for it)")
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):

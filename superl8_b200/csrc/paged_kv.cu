@@ -5,7 +5,7 @@
 // page and KV head; a value is code * scale.  block_table [B, max_pages] names the page of every page_size
 // tokens of a sequence.
 //
-// Append: block (page of a sequence, group of heads).  All new tokens of a page meet in one block, so its
+// Append: block (page of a sequence, head, K or V).  All new tokens of a page meet in one block, so its
 // scale needs no atomics and nothing depends on an order:
 //   scale' = max(scale, max|new| / 127, 2^-40)   (scale = 0 where the page holds no older token),
 //   code   = rint(x / scale'),   older codes -> rint(code * scale / scale')  when scale' > scale.
@@ -41,8 +41,7 @@ struct AppendArgs {
   const int32_t* new_lens;    // nullable: M
   int B, Hq, Hkv, M, D, page_shift, max_pages, num_pages, interleaved;
   int page_slots;             // pages one sequence's new tokens can touch
-  int heads_per_block, head_groups;
-  int64_t kv_blocks;
+  int64_t kv_units;           // (sequence, page, head): blocks that store K, and as many that store V
   int q_heads_per_block, q_head_groups;
 };
 
@@ -50,13 +49,14 @@ __device__ __forceinline__ int new_count(const AppendArgs& a, int b) {
   return a.new_lens ? min(max(__ldg(a.new_lens + b), 0), a.M) : a.M;
 }
 
-// Angles of VEC frequencies for new token i of sequence b whose place in the sequence is `place`.
-__device__ __forceinline__ void append_angles(const AppendArgs& a, int i0, int b, int i, int place, float (&c)[8], float (&s)[8]) {
+// Angles of 8 frequencies for new token i of sequence b whose place in the sequence is `place`.
+__device__ __forceinline__ void append_angles(const AppendArgs& a, const unsigned long long* table, int i0, int b, int i, int place,
+                                              float (&c)[8], float (&s)[8]) {
   if (a.f.positions) {
-    rope_angles<8>(a.f, i0, b, i, c, s);
+    rope_angles<8>(a.f, table, i0, b, i, c, s);
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) rope_angle((double)place, __ldg(a.f.inv_freq + i0 + e), c[e], s[e]);
+    for (int e = 0; e < 8; ++e) rope_angle(place, table[i0 + e], c[e], s[e]);
   }
 }
 
@@ -94,13 +94,13 @@ __device__ __forceinline__ void requantise(int8_t* codes, int bytes, float ratio
   }
 }
 
-// The role of a block that stores K and V: one page of one sequence, heads_per_block heads.
+// The role of a block that stores K or V: one page of one sequence and one head of one of the two.
 // NIT > 0: items (16 channels of a token) per thread, held in registers between the maximum and the
 // codes; NIT = 0: any number, read twice (the second time from L1 / L2).
-template <typename T, int NIT>
-__device__ void append_page(const AppendArgs& a, int64_t block, uint32_t* red) {
-  const int group = (int)(block % a.head_groups);
-  const int64_t rest = block / a.head_groups;
+template <typename T, int NIT, bool IS_K>
+__device__ void append_page(const AppendArgs& a, int64_t unit, uint32_t* red, const unsigned long long* table) {
+  const int h = (int)(unit % a.Hkv);
+  const int64_t rest = unit / a.Hkv;
   const int slot = (int)(rest % a.page_slots), b = (int)(rest / a.page_slots);
   const int len = __ldg(a.lens + b), n = new_count(a, b);
   const int page_size = 1 << a.page_shift;
@@ -114,105 +114,80 @@ __device__ void append_page(const AppendArgs& a, int64_t block, uint32_t* red) {
   const int page = __ldg(a.table + b * a.table_stride + page_no);
   if (page < 0 || page >= a.num_pages) return;                     // a page the cache does not have: nothing is stored
 
-  const int per_row = a.D / 16;
+  const PoolArgs& pool = IS_K ? a.k : a.v;
+  const int per_row = a.D / 16, row_shift = __ffs(per_row) - 1;    // D is a power of two
   const int items = (t1 - t0) * per_row;
   const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5;
   const int i_first = (int)(lo + t0 - start);                      // new-token index of place t0
-  const int h0 = group * a.heads_per_block, h1 = min(a.Hkv, h0 + a.heads_per_block);
-  constexpr int KEEP = NIT > 0 ? NIT : 1;
+  const bool interleaved = a.interleaved != 0;
+  const int64_t ph = (int64_t)page * a.Hkv + h;
+  int8_t* const codes = pool.codes + ph * page_size * a.D;
+  const T* x = reinterpret_cast<const T*>(pool.x) + b * pool.x_sb + h * pool.x_sh + i_first * pool.x_ss;
+  const float old = t0 > 0 ? pool.scale[ph] : 0.f;
 
-  float c[KEEP][8], s[KEEP][8];
+  // an item's 16 values, rotated
+  auto fetch = [&](int item, float (&u)[8], float (&w)[8]) {
+    const int row = item >> row_shift, j = item & (per_row - 1);
+    const bool turn = IS_K && j * 8 < a.f.half;
+    const int2 at = IS_K ? rope_item<8>(j, a.f.half, interleaved) : make_int2(16 * j, 16 * j + 8);
+    const Piece<T, 8> p0 = piece_load<T, 8>(x + row * pool.x_ss + at.x), p1 = piece_load<T, 8>(x + row * pool.x_ss + at.y);
+    float c[8], s[8];
+    if (turn) append_angles(a, table, j * 8, b, i_first + row, (int)lo + t0 + row, c, s);
+    p0.get(u);
+    p1.get(w);
+    if (turn) rope_turn<8>(u, w, c, s, interleaved);
+  };
+  auto put = [&](int item, const float (&u)[8], const float (&w)[8], float inv) {
+    const int row = item >> row_shift, j = item & (per_row - 1);
+    const int2 at = IS_K ? rope_item<8>(j, a.f.half, interleaved) : make_int2(16 * j, 16 * j + 8);
+    store_codes(codes + (int64_t)(t0 + row) * a.D, at, u, w, inv);
+  };
+  constexpr int KEEP = NIT > 0 ? NIT : 1;
+  float u[KEEP][8], w[KEEP][8];
+  uint32_t top = 0;
   if (NIT > 0) {
 #pragma unroll
-    for (int it = 0; it < KEEP; ++it) {
-      const int item = tid + it * threads, row = item / per_row, j = item - row * per_row;
-      if (item < items && j * 8 < a.f.half) append_angles(a, j * 8, b, i_first + row, (int)lo + t0 + row, c[it], s[it]);
+    for (int it = 0; it < KEEP; ++it)
+      if (tid + it * threads < items) {
+        fetch(tid + it * threads, u[it], w[it]);
+        top = max(top, abs_bits(u[it], w[it]));
+      }
+  } else {
+    for (int item = tid; item < items; item += threads) {
+      fetch(item, u[0], w[0]);
+      top = max(top, abs_bits(u[0], w[0]));
     }
   }
-  for (int h = h0; h < h1; ++h) {
-    const int64_t ph = (int64_t)page * a.Hkv + h;
-    const int64_t page_at = ph * page_size * a.D;
-    const T* kx = reinterpret_cast<const T*>(a.k.x) + b * a.k.x_sb + h * a.k.x_sh + i_first * a.k.x_ss;
-    const T* vx = reinterpret_cast<const T*>(a.v.x) + b * a.v.x_sb + h * a.v.x_sh + i_first * a.v.x_ss;
-    float ku[KEEP][8], kw[KEEP][8];
-    Piece<T, 8> vu[KEEP], vw[KEEP];
-    uint32_t ktop = 0, vtop = 0;
-    // one item: load, rotate, largest magnitudes
-    auto fetch = [&](int item, float (&u)[8], float (&w)[8], Piece<T, 8>& y, Piece<T, 8>& z, const float (&cc)[8], const float (&ss)[8]) {
-      const int row = item / per_row, j = item - row * per_row;
-      const int2 at = rope_item<8>(j, a.f.half, a.interleaved != 0);
-      const Piece<T, 8> p0 = piece_load<T, 8>(kx + row * a.k.x_ss + at.x), p1 = piece_load<T, 8>(kx + row * a.k.x_ss + at.y);
-      y = piece_load<T, 8>(vx + row * a.v.x_ss + 16 * j);
-      z = piece_load<T, 8>(vx + row * a.v.x_ss + 16 * j + 8);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) { u[e] = to_f32<T>(p0.v[e]); w[e] = to_f32<T>(p1.v[e]); }
-      if (j * 8 < a.f.half) rope_turn<8>(u, w, cc, ss, a.interleaved != 0);
-      ktop = max(ktop, abs_bits(u, w));
-      float f0[8], f1[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) { f0[e] = to_f32<T>(y.v[e]); f1[e] = to_f32<T>(z.v[e]); }
-      vtop = max(vtop, abs_bits(f0, f1));
-    };
-    auto put = [&](int item, const float (&u)[8], const float (&w)[8], const Piece<T, 8>& y, const Piece<T, 8>& z, float kinv, float vinv) {
-      const int row = item / per_row, j = item - row * per_row;
-      const int64_t at = page_at + (int64_t)(t0 + row) * a.D;
-      store_codes(a.k.codes + at, rope_item<8>(j, a.f.half, a.interleaved != 0), u, w, kinv);
-      float f0[8], f1[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) { f0[e] = to_f32<T>(y.v[e]); f1[e] = to_f32<T>(z.v[e]); }
-      store_codes(a.v.codes + at, make_int2(16 * j, 16 * j + 8), f0, f1, vinv);
-    };
-    auto angles_again = [&](int item, float (&cc)[8], float (&ss)[8]) {
-      const int row = item / per_row, j = item - row * per_row;
-      if (j * 8 < a.f.half) append_angles(a, j * 8, b, i_first + row, (int)lo + t0 + row, cc, ss);
-    };
-    if (NIT > 0) {
-#pragma unroll
-      for (int it = 0; it < KEEP; ++it)
-        if (tid + it * threads < items) fetch(tid + it * threads, ku[it], kw[it], vu[it], vw[it], c[it], s[it]);
-    } else {
-      for (int item = tid; item < items; item += threads) {
-        angles_again(item, c[0], s[0]);
-        fetch(item, ku[0], kw[0], vu[0], vw[0], c[0], s[0]);
-      }
-    }
-    ktop = __reduce_max_sync(0xffffffffu, ktop);
-    vtop = __reduce_max_sync(0xffffffffu, vtop);
-    if (threads > 32) {
-      __syncthreads();                                             // the previous head's readers are done
-      if (lane == 0) { red[2 * warp] = ktop; red[2 * warp + 1] = vtop; }
-      __syncthreads();
-      for (int w = 0; w < threads / 32; ++w) { ktop = max(ktop, red[2 * w]); vtop = max(vtop, red[2 * w + 1]); }
-    }
-    const float k_old = t0 > 0 ? a.k.scale[ph] : 0.f, v_old = t0 > 0 ? a.v.scale[ph] : 0.f;
-    // as bits again: a NaN scale stays
-    auto larger = [](float old, uint32_t top) {
-      const uint32_t now = max(__float_as_uint(old) & 0x7fffffffu, __float_as_uint(__fdiv_rn(__uint_as_float(top), 127.f)));
-      return __uint_as_float(max(now, __float_as_uint(kScaleFloor)));
-    };
-    const float k_now = larger(k_old, ktop), v_now = larger(v_old, vtop);
-    const float kinv = 1.f / k_now, vinv = 1.f / v_now;
-    if (NIT > 0) {
-#pragma unroll
-      for (int it = 0; it < KEEP; ++it)
-        if (tid + it * threads < items) put(tid + it * threads, ku[it], kw[it], vu[it], vw[it], kinv, vinv);
-    } else {
-      for (int item = tid; item < items; item += threads) {
-        angles_again(item, c[0], s[0]);
-        fetch(item, ku[0], kw[0], vu[0], vw[0], c[0], s[0]);
-        put(item, ku[0], kw[0], vu[0], vw[0], kinv, vinv);
-      }
-    }
-    if (t0 > 0 && k_now != k_old) requantise(a.k.codes + page_at, t0 * a.D, __fdiv_rn(k_old, k_now), tid, threads);
-    if (t0 > 0 && v_now != v_old) requantise(a.v.codes + page_at, t0 * a.D, __fdiv_rn(v_old, v_now), tid, threads);
-    if (threads > 32) __syncthreads(); else __syncwarp();          // every thread has read the old scales
-    if (tid == 0) { a.k.scale[ph] = k_now; a.v.scale[ph] = v_now; }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (threads > 32) {
+    if (lane == 0) red[warp] = top;
+    __syncthreads();
+    for (int i = 0; i < threads / 32; ++i) top = max(top, red[i]);
+  } else {
+    __syncwarp();
   }
+  // as bits again: a NaN scale stays
+  uint32_t bits = max(__float_as_uint(old) & 0x7fffffffu, __float_as_uint(__fdiv_rn(__uint_as_float(top), 127.f)));
+  const float now = __uint_as_float(max(bits, __float_as_uint(kScaleFloor)));
+  const float inv = 1.f / now;
+  if (NIT > 0) {
+#pragma unroll
+    for (int it = 0; it < KEEP; ++it)
+      if (tid + it * threads < items) put(tid + it * threads, u[it], w[it], inv);
+  } else {
+    for (int item = tid; item < items; item += threads) {
+      fetch(item, u[0], w[0]);
+      put(item, u[0], w[0], inv);
+    }
+  }
+  if (t0 > 0 && now != old) requantise(codes, t0 * a.D, __fdiv_rn(old, now), tid, threads);
+  // the other threads of a wide block have read the old scale: they passed the barrier above
+  if (tid == 0) pool.scale[ph] = now;
 }
 
 // The role of a block that rotates Q: as rope.cu, rows past new_lens are written as zeros.
 template <typename T>
-__device__ void append_query(const AppendArgs& a, int64_t block) {
+__device__ void append_query(const AppendArgs& a, int64_t block, const unsigned long long* table) {
   const int group = (int)(block % a.q_head_groups);
   const int per_row = a.D / 16;
   const int64_t item = block / a.q_head_groups * blockDim.x + threadIdx.x;
@@ -223,70 +198,75 @@ __device__ void append_query(const AppendArgs& a, int64_t block) {
   const int n = new_count(a, b);
   const bool real = i < n, turn = real && j * 8 < a.f.half;
   const int2 at = rope_item<8>(j, a.f.half, a.interleaved != 0);
+  const int h0 = group * a.q_heads_per_block, h1 = min(a.Hq, h0 + a.q_heads_per_block);
+  const T* x = reinterpret_cast<const T*>(a.q) + b * a.q_sb + i * a.q_ss + h0 * a.q_sh;
+  T* y = reinterpret_cast<T*>(a.q_out) + b * a.qo_sb + i * a.qo_ss + h0 * a.qo_sh;
   float c[8], s[8];
-  if (turn) append_angles(a, j * 8, b, i, __ldg(a.lens + b) - n + i, c, s);
-  const int h1 = min(a.Hq, (group + 1) * a.q_heads_per_block);
-#pragma unroll 4
-  for (int h = group * a.q_heads_per_block; h < h1; ++h) {
+  if (turn) append_angles(a, table, j * 8, b, i, __ldg(a.lens + b) - n + i, c, s);
+#pragma unroll 2
+  for (int h = h0; h < h1; ++h) {
     Piece<T, 8> p0, p1;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) p0.v[e] = p1.v[e] = from_f32<T>(0.f);
+    p0.zero();
+    p1.zero();
     if (real) {
-      const T* x = reinterpret_cast<const T*>(a.q) + b * a.q_sb + h * a.q_sh + i * a.q_ss;
       p0 = piece_load<T, 8>(x + at.x);
       p1 = piece_load<T, 8>(x + at.y);
     }
     if (turn) {
       float u[8], w[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) { u[e] = to_f32<T>(p0.v[e]); w[e] = to_f32<T>(p1.v[e]); }
+      p0.get(u);
+      p1.get(w);
       rope_turn<8>(u, w, c, s, a.interleaved != 0);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) { p0.v[e] = from_f32<T>(u[e]); p1.v[e] = from_f32<T>(w[e]); }
+      p0.put(u);
+      p1.put(w);
     }
-    T* y = reinterpret_cast<T*>(a.q_out) + b * a.qo_sb + h * a.qo_sh + i * a.qo_ss;
-    *reinterpret_cast<Piece<T, 8>*>(y + at.x) = p0;
-    *reinterpret_cast<Piece<T, 8>*>(y + at.y) = p1;
+    p0.store(y + at.x);
+    p1.store(y + at.y);
+    x += a.q_sh;
+    y += a.qo_sh;
   }
 }
 
 template <typename T, int NIT>
-__global__ void __launch_bounds__(512) append_kernel(const AppendArgs a) {
-  __shared__ uint32_t red[32];
-  if ((int64_t)blockIdx.x < a.kv_blocks) append_page<T, NIT>(a, blockIdx.x, red);
-  else append_query<T>(a, (int64_t)blockIdx.x - a.kv_blocks);
+__global__ void __launch_bounds__(256, 3) append_kernel(const AppendArgs a) {
+  __shared__ uint32_t red[8];
+  __shared__ unsigned long long table[128];   // D <= 256
+  const int64_t block = blockIdx.x;
+  const bool v_role = block >= a.kv_units && block < 2 * a.kv_units;
+  if (a.f.half > 0 && !v_role) {
+    rope_table(table, a.f);
+    if (blockDim.x > 32) __syncthreads(); else __syncwarp();
+  }
+  if (block < a.kv_units) append_page<T, NIT, true>(a, block, red, table);
+  else if (v_role) append_page<T, NIT, false>(a, block - a.kv_units, red, table);
+  else append_query<T>(a, block - 2 * a.kv_units, table);
 }
 
 template <typename T>
 int launch_append(AppendArgs a, cudaStream_t stream) {
   const int page_size = 1 << a.page_shift;
   const int rows = a.M < page_size ? a.M : page_size;
-  const int items = rows * (a.D / 16);                      // of one head's K (and as many of V)
-  // One warp serves a single token's heads; a full page of 64 x 128 takes 256 threads with two items each.
-  // Above 1024 items (page 128 x 256 and larger) the rows are read twice instead of held.
+  const int items = rows * (a.D / 16);
+  // One warp serves a single token; a full page of 64 x 128 takes 256 threads with two items each.  Above
+  // 512 items (pages of 128 x 128 and larger) the rows are read twice instead of held.
   int threads = 32;
-  while (threads < 512 && threads * 2 < items) threads *= 2;
+  while (threads < 256 && threads < items) threads *= 2;
   const int nit = (items + threads - 1) / threads;
   a.page_slots = (a.M + page_size - 2) / page_size + 1;
   if (a.page_slots > a.max_pages) a.page_slots = a.max_pages;
-  // Heads share the angles of a block's tokens as long as eight blocks per SM are left.
-  const int64_t pages = (int64_t)a.B * a.page_slots;
-  int64_t groups = pages > 0 ? (kNumSms * 8 + pages - 1) / pages : 1;
-  if (groups > a.Hkv) groups = a.Hkv;
-  a.heads_per_block = (int)((a.Hkv + groups - 1) / groups);
-  a.head_groups = (a.Hkv + a.heads_per_block - 1) / a.heads_per_block;
-  a.kv_blocks = pages * a.head_groups;
+  a.kv_units = (int64_t)a.B * a.page_slots * a.Hkv;
   int64_t q_blocks = 0;
   if (a.q) {
-    const int64_t q_items = (int64_t)a.B * a.M * (a.D / 16);
-    const int64_t gx = (q_items + threads - 1) / threads;
-    groups = (kNumSms * 16 + gx - 1) / gx;
-    if (groups > a.Hq) groups = a.Hq;
+    // the heads of a block share the angles: at least four of them unless that leaves SMs idle
+    const int64_t gx = ((int64_t)a.B * a.M * (a.D / 16) + threads - 1) / threads;
+    int64_t groups = (kNumSms * 16 + gx - 1) / gx, most = (a.Hq + 3) / 4;
+    if (gx * most < kNumSms * 8) most = a.Hq;
+    if (groups > most) groups = most;
     a.q_heads_per_block = (int)((a.Hq + groups - 1) / groups);
     a.q_head_groups = (a.Hq + a.q_heads_per_block - 1) / a.q_heads_per_block;
     q_blocks = gx * a.q_head_groups;
   }
-  const int64_t blocks = a.kv_blocks + q_blocks;
+  const int64_t blocks = 2 * a.kv_units + q_blocks;
   if (blocks == 0) return SL8_OK;
   if (blocks > 0x7fffffffll) return SL8_ERR_TOO_LARGE;
   if (nit <= 1) append_kernel<T, 1><<<(unsigned)blocks, threads, 0, stream>>>(a);

@@ -3,8 +3,8 @@
 //
 // HBM bound: every element is read once and written once, 2 e bytes.  A thread owns one item -- 2 VEC
 // channels of one token that pair with one another -- works out its VEC angles once and walks the
-// heads with them, so the angles (64-bit products, sincospif) are shared by all heads of a block's
-// group and the loads of four heads are in flight together.
+// heads with them, so the angles (fixed-point products and two short series, sl8_rope.cuh) are shared by
+// all heads of a block's group and the loads of four heads are in flight together.
 #include "sl8_rope.cuh"
 
 namespace sl8 {
@@ -24,59 +24,72 @@ struct RopeArgs {
 };
 
 constexpr int kRopeThreads = 256;
-constexpr int kRopeUnroll = 4;
+
+// U heads in flight per thread; four blocks per SM where an item's pieces leave the registers for it.
+template <typename T, int VEC>
+struct RopeCfg {
+  static constexpr int BYTES = sizeof(T) * VEC;
+  static constexpr int U = BYTES > 16 ? 2 : 4;
+  static constexpr int BLOCKS = BYTES > 16 ? 2 : 3;
+};
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
+__global__ void __launch_bounds__(kRopeThreads, RopeCfg<T, VEC>::BLOCKS) rope_kernel(const RopeArgs a) {
+  constexpr int U = RopeCfg<T, VEC>::U;
+  extern __shared__ unsigned long long table[];
   const int64_t item = (int64_t)blockIdx.x * kRopeThreads + threadIdx.x;
   const int64_t token = item / a.items;
-  if (token >= a.tokens) return;
+  const bool real = token < a.tokens;
   const int j = (int)(item - token * a.items);
   const int64_t b = token / a.S, s = token - b * a.S;
   const bool turn = j * VEC < a.f.half;
-  const int2 at = rope_item<VEC>(j, a.f.half, a.interleaved != 0);
+  const bool interleaved = a.interleaved != 0;
+  const int2 at = rope_item<VEC>(j, a.f.half, interleaved);
   const int h0 = blockIdx.y * a.heads_per_block, h1 = min(a.H, h0 + a.heads_per_block);
 
-  Piece<T, VEC> p0[kRopeUnroll], p1[kRopeUnroll];
-  auto load = [&](int h, Piece<T, VEC>& u, Piece<T, VEC>& w) {
-    const RopeTensor& t = h < a.Hq ? a.q : a.k;
-    const T* x = reinterpret_cast<const T*>(t.x) + b * t.x_sb + (h < a.Hq ? h : h - a.Hq) * t.x_sh + s * t.x_ss;
-    u = piece_load<T, VEC>(x + at.x);
-    w = piece_load<T, VEC>(x + at.y);
-  };
-  auto store = [&](int h, const Piece<T, VEC>& u, const Piece<T, VEC>& w) {
-    const RopeTensor& t = h < a.Hq ? a.q : a.k;
-    T* y = reinterpret_cast<T*>(t.y) + b * t.y_sb + (h < a.Hq ? h : h - a.Hq) * t.y_sh + s * t.y_ss;
-    *reinterpret_cast<Piece<T, VEC>*>(y + at.x) = u;
-    *reinterpret_cast<Piece<T, VEC>*>(y + at.y) = w;
-  };
-  // the first heads' loads go out before the angles are worked out
-#pragma unroll
-  for (int i = 0; i < kRopeUnroll; ++i)
-    if (h0 + i < h1) load(h0 + i, p0[i], p1[i]);
+  rope_table(table, a.f);
+  __syncthreads();
+  if (!real) return;
   float c[VEC], sn[VEC];
-  if (turn) rope_angles<VEC>(a.f, j * VEC, b, s, c, sn);
-  for (int h = h0; h < h1; h += kRopeUnroll) {
-    if (h != h0) {
-#pragma unroll
-      for (int i = 0; i < kRopeUnroll; ++i)
-        if (h + i < h1) load(h + i, p0[i], p1[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < kRopeUnroll; ++i) {
-      if (h + i < h1) {
-        if (turn) {
-          float u[VEC], w[VEC];
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) { u[e] = to_f32<T>(p0[i].v[e]); w[e] = to_f32<T>(p1[i].v[e]); }
-          rope_turn<VEC>(u, w, c, sn, a.interleaved != 0);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) { p0[i].v[e] = from_f32<T>(u[e]); p1[i].v[e] = from_f32<T>(w[e]); }
-        }
-        store(h + i, p0[i], p1[i]);
+  if (turn) rope_angles<VEC>(a.f, table, j * VEC, b, s, c, sn);
+
+  auto heads = [&](const RopeTensor& t, int from, int to) {
+    const T* x = reinterpret_cast<const T*>(t.x) + b * t.x_sb + s * t.x_ss + from * t.x_sh;
+    T* y = reinterpret_cast<T*>(t.y) + b * t.y_sb + s * t.y_ss + from * t.y_sh;
+    auto one = [&](Piece<T, VEC>& p0, Piece<T, VEC>& p1, T* dst) {
+      if (turn) {
+        float u[VEC], w[VEC];
+        p0.get(u);
+        p1.get(w);
+        rope_turn<VEC>(u, w, c, sn, interleaved);
+        p0.put(u);
+        p1.put(w);
       }
+      p0.store(dst + at.x);
+      p1.store(dst + at.y);
+    };
+    int n = to - from;
+    for (; n >= U; n -= U) {
+      Piece<T, VEC> p0[U], p1[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        p0[i] = piece_load<T, VEC>(x + i * t.x_sh + at.x);
+        p1[i] = piece_load<T, VEC>(x + i * t.x_sh + at.y);
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i) one(p0[i], p1[i], y + i * t.y_sh);
+      x += U * t.x_sh;
+      y += U * t.y_sh;
     }
-  }
+    for (; n > 0; --n) {
+      Piece<T, VEC> p0 = piece_load<T, VEC>(x + at.x), p1 = piece_load<T, VEC>(x + at.y);
+      one(p0, p1, y);
+      x += t.x_sh;
+      y += t.y_sh;
+    }
+  };
+  if (h0 < a.Hq) heads(a.q, h0, min(h1, a.Hq));
+  if (h1 > a.Hq) heads(a.k, max(h0, a.Hq) - a.Hq, h1 - a.Hq);
 }
 
 template <typename T, int VEC>
@@ -84,13 +97,15 @@ int launch_rope(RopeArgs a, int D, cudaStream_t stream) {
   a.items = D / (2 * VEC);
   const int64_t gx = (a.tokens * a.items + kRopeThreads - 1) / kRopeThreads;
   if (gx > 0x7fffffffll) return SL8_ERR_TOO_LARGE;
-  // As many heads per block as still leave eight blocks per SM: the angles are worked out once per block.
-  int64_t groups = (kNumSms * 8 + gx - 1) / gx;
-  if (groups > a.H) groups = a.H;
+  // A block's heads share the angles (as much work as four heads' products): at least four of them, unless
+  // that leaves SMs idle, and few enough for six waves of blocks.
+  int64_t groups = (kNumSms * 18 + gx - 1) / gx, most = (a.H + 3) / 4;
+  if (gx * most < kNumSms * 3) most = a.H;
+  if (groups > most) groups = most;
   a.heads_per_block = (int)((a.H + groups - 1) / groups);
   const unsigned gy = (unsigned)((a.H + a.heads_per_block - 1) / a.heads_per_block);
   if (gy > 65535u) return SL8_ERR_TOO_LARGE;
-  rope_kernel<T, VEC><<<dim3((unsigned)gx, gy), kRopeThreads, 0, stream>>>(a);
+  rope_kernel<T, VEC><<<dim3((unsigned)gx, gy), kRopeThreads, a.f.half * 8, stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? SL8_OK : SL8_ERR_CUDA;
 }
 
@@ -128,7 +143,7 @@ using namespace sl8;
 extern "C" int sl8_rope(const sl8_rope_params* p, void* stream) {
   if (p == nullptr) return SL8_ERR_NULL;
   if (p->B < 0 || p->Hq < 0 || p->Hkv < 0 || p->S < 0 || p->n_axes < 1) return SL8_ERR_BAD_SHAPE;
-  if (p->D < 2 || p->D % 2 != 0 || p->rot < 0 || p->rot > p->D || p->rot % 2 != 0) return SL8_ERR_BAD_SHAPE;
+  if (p->D < 2 || p->D > 8192 || p->D % 2 != 0 || p->rot < 0 || p->rot > p->D || p->rot % 2 != 0) return SL8_ERR_BAD_SHAPE;
   if (p->dtype != SL8_F16 && p->dtype != SL8_BF16 && p->dtype != SL8_F32) return SL8_ERR_BAD_DTYPE;
   const int Hq = p->q ? p->Hq : 0, Hkv = p->k ? p->Hkv : 0;
   if ((int64_t)p->B * p->S * (Hq + Hkv) == 0) return SL8_OK;

@@ -129,6 +129,47 @@ std::tuple<Tensor, OptTensor> rope(const Tensor& q_in, const OptTensor& k_in, co
   return {q_out, k_in.has_value() ? OptTensor(k_out) : OptTensor()};
 }
 
+// The rotation is linear and orthogonal: its gradient is the rotation by the opposite angle, itself
+// differentiable the same way.
+struct RopeFunction : public torch::autograd::Function<RopeFunction> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const OptTensor& k,
+                                                const Tensor& positions, const Tensor& inv_freq, const OptTensor& freq_axis,
+                                                bool interleaved, bool inverse) {
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({positions, inv_freq, freq_axis.has_value() ? *freq_axis : Tensor()});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["inverse"] = inverse;
+    const auto r = rope(q, k, positions, inv_freq, freq_axis, interleaved, inverse);
+    if (!k.has_value()) return {std::get<0>(r)};
+    return {std::get<0>(r), *std::get<1>(r)};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, const torch::autograd::variable_list& grads) {
+    const auto saved = ctx->get_saved_variables();
+    const bool interleaved = ctx->saved_data["interleaved"].toBool(), inverse = ctx->saved_data["inverse"].toBool();
+    const OptTensor axis = saved[2].defined() ? OptTensor(saved[2]) : OptTensor();
+    Tensor dq = grads[0], dk = grads.size() > 1 ? grads[1] : Tensor();
+    if (dq.defined() || dk.defined()) {
+      const bool both = dq.defined() && dk.defined();
+      const auto r = RopeFunction::apply(dq.defined() ? dq : dk, both ? OptTensor(dk) : OptTensor(), saved[0], saved[1], axis, interleaved,
+                                         !inverse);
+      if (both) { dq = r[0]; dk = r[1]; }
+      else if (dq.defined()) dq = r[0];
+      else dk = r[0];
+    }
+    return {dq, dk, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, OptTensor> apply_rope(const Tensor& q, const OptTensor& k, const Tensor& positions, const Tensor& inv_freq,
+                                         const OptTensor& freq_axis, bool interleaved) {
+  TORCH_CHECK(!inv_freq.requires_grad(), "superl8_b200 apply_rope: inv_freq is a constant (no gradient is computed for it)");
+  if (!(at::GradMode::is_enabled() && (q.requires_grad() || (k.has_value() && k->requires_grad()))))
+    return rope(q, k, positions, inv_freq, freq_axis, interleaved, false);
+  const auto r = RopeFunction::apply(q, k, positions, inv_freq, freq_axis, interleaved, false);
+  return {r[0], k.has_value() ? OptTensor(r[1]) : OptTensor()};
+}
+
 // The cache's tensors and a batch's table and lengths.
 sl8_paged_cache cache_of(const Tensor& k_i8, const Tensor& k_scale, const Tensor& v_i8, const Tensor& v_scale, const Tensor& table,
                          const Tensor& lens, const char* what) {
@@ -168,6 +209,7 @@ const int32_t* lens_of(const OptTensor& t, const Tensor& like, int64_t B, const 
 OptTensor kv_append_paged(const Tensor& k_in, const Tensor& v_in, const Tensor& k_i8, const Tensor& k_scale, const Tensor& v_i8,
                           const Tensor& v_scale, const Tensor& table, const Tensor& lens, const OptTensor& new_lens, const OptTensor& q_in,
                           const OptTensor& positions, const OptTensor& inv_freq, const OptTensor& freq_axis, bool interleaved) {
+  const at::NoGradGuard no_grad;   // the cache operators carry no gradient
   const char* what = "kv_append_paged";
   const sl8_paged_cache c = cache_of(k_i8, k_scale, v_i8, v_scale, table, lens, what);
   check_on(k_in, k_i8, what);
@@ -229,6 +271,7 @@ std::tuple<Tensor, Tensor> kv_read_paged(const Tensor& k_i8, const Tensor& k_sca
 Tensor attn_paged(const Tensor& q_in, const Tensor& k_i8, const Tensor& k_scale, const Tensor& v_i8, const Tensor& v_scale,
                   const Tensor& table, const Tensor& lens, const c10::optional<double>& scale, bool causal, int64_t window_left,
                   const OptTensor& query_lens, int64_t max_context_len) {
+  const at::NoGradGuard no_grad;   // the cache operators carry no gradient
   const char* what = "attn_paged_cached";
   const sl8_paged_cache c = cache_of(k_i8, k_scale, v_i8, v_scale, table, lens, what);
   check_on(q_in, k_i8, what);
@@ -262,6 +305,8 @@ void bind_paged(pybind11::module_& m) {
   namespace py = pybind11;
   m.def("rope", &rope, py::arg("q"), py::arg("k"), py::arg("positions"), py::arg("inv_freq"), py::arg("freq_axis"), py::arg("interleaved"),
         py::arg("inverse"));
+  m.def("apply_rope", &apply_rope, py::arg("q"), py::arg("k"), py::arg("positions"), py::arg("inv_freq"), py::arg("freq_axis"),
+        py::arg("interleaved"));
   m.def("kv_append_paged", &kv_append_paged, py::arg("k"), py::arg("v"), py::arg("k_i8"), py::arg("k_scale"), py::arg("v_i8"),
         py::arg("v_scale"), py::arg("block_table"), py::arg("context_lens"), py::arg("new_lens"), py::arg("q"), py::arg("positions"),
         py::arg("inv_freq"), py::arg("freq_axis"), py::arg("interleaved"));

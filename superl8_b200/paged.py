@@ -35,7 +35,6 @@ def empty_paged_cache(num_pages: int, num_kv_heads: int, page_size: int, head_di
     return codes[0], scales[0], codes[1], scales[1]
 
 
-@torch.no_grad()
 def kv_append_paged(k, v, k_i8, k_scale, v_i8, v_scale, block_table, context_lens, *, new_lens=None, q=None, positions=None,
                     inv_freq=None, freq_axis=None, interleaved: bool = False):
     """Stores the newest tokens of every sequence: k, v fp16/bf16 [B, H_kv, M, D] (strided views are taken in
@@ -55,7 +54,6 @@ def kv_append_paged(k, v, k_i8, k_scale, v_i8, v_scale, block_table, context_len
                               freq_axis, interleaved)
 
 
-@torch.no_grad()
 def kv_read_paged(k_i8, k_scale, v_i8, v_scale, block_table, context_lens, num_tokens: int, *, first=None,
                   dtype=torch.float16):
     """The cache's values as (k, v) fp16 / bf16 [B, H_kv, num_tokens, D]: row j is token ``first[b] + j``
@@ -64,7 +62,6 @@ def kv_read_paged(k_i8, k_scale, v_i8, v_scale, block_table, context_lens, num_t
     return _C.kv_read_paged(k_i8, k_scale, v_i8, v_scale, block_table, context_lens, num_tokens, first, dtype)
 
 
-@torch.no_grad()
 def attn_paged_cached(q, k_i8, k_scale, v_i8, v_scale, block_table, context_lens, *, scale: float | None = None,
                       causal: bool = True, window_left: int = -1, query_lens=None, max_context_len: int | None = None):
     """softmax(scale q.K^T) V over the paged cache; q fp16/bf16 [B, H_q, M, D] (rotated where the cache's
