@@ -22,6 +22,7 @@
 #include "sl8_paged.cuh"
 #include "sl8_mma.cuh"
 
+#include <algorithm>
 #include <atomic>
 
 namespace sl8 {
@@ -107,7 +108,7 @@ __device__ __forceinline__ uint32_t tile_offset(int r, int c) {
 
 // Keys per warp and step: 32 (two 16-key tiles share the maximum, the rescaling and the loop) where the
 // accumulators leave the registers for it and the ring the space, else 16.
-__host__ __device__ constexpr int chunk_shift_of(int D, int ng) { return D == 256 || (D >= 64 && ng == 4) ? 4 : 5; }
+__host__ __device__ constexpr int chunk_shift_of(int D, int ng) { return D == 256 || (D >= 64 && ng >= 3) ? 4 : 5; }
 
 // Most groups of 8 query rows a warp can accumulate: D / 4 registers a thread each.
 __host__ __device__ constexpr int groups_of(int D) { return D == 256 ? 2 : 4; }
@@ -350,32 +351,47 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
         iv[h] = empty ? 0.f : rcp_approx(scales.y);
       }
 
-      uint32_t kf[T][D / 32][4];
+      // ---- S^T = K . Q^T: keys g, g + 8 of a tile, rows 2t, 2t + 1.  All tiles, groups and planes step
+      // through the channels together: 2 T NG independent accumulations hide the MMA's latency ----
+      int hi[T][NG][4], lo[T][NG][4];
 #pragma unroll
       for (int h = 0; h < T; ++h)
 #pragma unroll
-        for (int w = 0; w < D / 32; ++w) ldmatrix_x4(kf[h][w], base + h * C::TILE + tile_offset<D>(m_row, 2 * w + m_piece));
-      uint32_t pb[NG][T][2];
+        for (int ng = 0; ng < NG; ++ng)
 #pragma unroll
-      for (int ng = 0; ng < NG; ++ng) {
-        // ---- S^T = K . Q^T: keys g, g + 8 of a tile, rows 2t, 2t + 1 ----
-        float x[T][4];
+          for (int e = 0; e < 4; ++e) hi[h][ng][e] = lo[h][ng][e] = 0;
+      uint32_t kf[T][D / 32][4];
 #pragma unroll
-        for (int h = 0; h < T; ++h) {
-          int hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+      for (int w = 0; w < D / 32; ++w)
 #pragma unroll
-          for (int w = 0; w < D / 32; ++w) {
-            uint4 q4;
-            if constexpr (C::Q_REGS) q4 = qr[ng][w];
-            else q4 = my_q[(ng * (D / 32) + w) * 32];
-            mma_s8_16832(hi, kf[h][w], q4.x, q4.y);
-            mma_s8_16832(lo, kf[h][w], q4.z, q4.w);
+        for (int h = 0; h < T; ++h) ldmatrix_x4(kf[h][w], base + h * C::TILE + tile_offset<D>(m_row, 2 * w + m_piece));
+#pragma unroll
+      for (int w = 0; w < D / 32; ++w) {
+#pragma unroll
+        for (int ng = 0; ng < NG; ++ng) {
+          uint4 q4;
+          if constexpr (C::Q_REGS) q4 = qr[ng][w];
+          else q4 = my_q[(ng * (D / 32) + w) * 32];
+#pragma unroll
+          for (int h = 0; h < T; ++h) {
+            mma_s8_16832(hi[h][ng], kf[h][w], q4.x, q4.y);
+            mma_s8_16832(lo[h][ng], kf[h][w], q4.z, q4.w);
           }
+        }
+      }
+      float x[T][NG][4];
+#pragma unroll
+      for (int h = 0; h < T; ++h)
+#pragma unroll
+        for (int ng = 0; ng < NG; ++ng) {
           const float f0 = row_scale[ng][0] * ks[h], f1 = row_scale[ng][1] * ks[h];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[h][e] = fmaf((float)(hi[e] * 128 + lo[e]), e & 1 ? f1 : f0, lv[h]);
+          for (int e = 0; e < 4; ++e)
+            x[h][ng][e] = fmaf((float)(hi[h][ng][e] * 128 + lo[h][ng][e]), e & 1 ? f1 : f0, lv[h]);
         }
-        if (!whole) {
+      if (!whole) {
+#pragma unroll
+        for (int ng = 0; ng < NG; ++ng)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int place = s.place + (r_first + ng * 8 + 2 * t + e) / a.G;
@@ -385,24 +401,32 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
 #pragma unroll
               for (int k8 = 0; k8 < 2; ++k8) {
                 const int key = key0 + 16 * h + 8 * k8 + g;
-                if (key >= to || key < from) x[h][2 * k8 + e] = -INFINITY;
+                if (key >= to || key < from) x[h][ng][2 * k8 + e] = -INFINITY;
               }
           }
+      }
+      // ---- reference, weights, row sums ----
+      float mx[NG][2];
+      bool grown = false;
+#pragma unroll
+      for (int ng = 0; ng < NG; ++ng)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          mx[ng][e] = fmaxf(x[0][ng][e], x[0][ng][e + 2]);
+          if constexpr (T == 2) mx[ng][e] = max3f(mx[ng][e], x[1][ng][e], x[1][ng][e + 2]);
+          grown |= mx[ng][e] > m_run[ng][e] + kSlack;
         }
-        // ---- reference, weights, row sums ----
-        float mx[2] = {fmaxf(x[0][0], x[0][2]), fmaxf(x[0][1], x[0][3])};
-        if constexpr (T == 2) {
-          mx[0] = max3f(mx[0], x[1][0], x[1][2]);
-          mx[1] = max3f(mx[1], x[1][1], x[1][3]);
-        }
-        if (__any_sync(0xffffffffu, mx[0] > m_run[ng][0] + kSlack || mx[1] > m_run[ng][1] + kSlack)) {
+      if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+        for (int ng = 0; ng < NG; ++ng) {
           float f[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 4));
-            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 8));
-            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 16));
-            const float m = fmaxf(m_run[ng][e], mx[e]);
+            float top = mx[ng][e];
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            const float m = fmaxf(m_run[ng][e], top);
             f[e] = ex2_approx(m_run[ng][e] - m);
             m_run[ng][e] = m;
             l_run[ng][e] *= f[e];
@@ -415,16 +439,26 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
             o[ng][d][3] *= f[1];
           }
         }
-#pragma unroll
-        for (int h = 0; h < T; ++h) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[h][e] = ex2_approx(x[h][e] - m_run[ng][e & 1]);
-          l_run[ng][0] = fmaf(x[h][0] + x[h][2], iv[h], l_run[ng][0]);
-          l_run[ng][1] = fmaf(x[h][1] + x[h][3], iv[h], l_run[ng][1]);
-          pb[ng][h][0] = transpose8x8(pack2<__half>(x[h][0], x[h][1]));
-          pb[ng][h][1] = transpose8x8(pack2<__half>(x[h][2], x[h][3]));
-        }
       }
+      uint32_t pb[NG][T][2];
+#pragma unroll
+      for (int h = 0; h < T; ++h)
+#pragma unroll
+        for (int ng = 0; ng < NG; ++ng) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[h][ng][e] = ex2_approx(x[h][ng][e] - m_run[ng][e & 1]);
+          l_run[ng][0] = fmaf(x[h][ng][0] + x[h][ng][2], iv[h], l_run[ng][0]);
+          l_run[ng][1] = fmaf(x[h][ng][1] + x[h][ng][3], iv[h], l_run[ng][1]);
+          pb[ng][h][0] = pack2<__half>(x[h][ng][0], x[h][ng][1]);
+          pb[ng][h][1] = pack2<__half>(x[h][ng][2], x[h][ng][3]);
+        }
+#pragma unroll
+      for (int h = 0; h < T; ++h)
+#pragma unroll
+        for (int ng = 0; ng < NG; ++ng) {
+          pb[ng][h][0] = transpose8x8(pb[ng][h][0]);
+          pb[ng][h][1] = transpose8x8(pb[ng][h][1]);
+        }
       // ---- O^T += V^T . P^T.  A transposing ldmatrix hands out byte pairs of two neighbouring channels for
       // keys 2t, 2t + 1; widened exactly ((b ^ 0x80) | 0x6400 is 1152 + b), channel 2g feeds row g of the
       // tile and channel 2g + 1 row g + 8 ----
@@ -435,19 +469,21 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
         return *reinterpret_cast<const uint32_t*>(&h);
       };
 #pragma unroll
-      for (int h = 0; h < T; ++h)
+      for (int h = 0; h < T; ++h) {
+        uint32_t r[D / 32][4];
 #pragma unroll
-        for (int w = 0; w < D / 32; ++w) {
-          uint32_t r[4];
-          ldmatrix_x4_trans(r, base + h * C::TILE + 16 * D + tile_offset<D>(m_row, 2 * w + m_piece));
+        for (int w = 0; w < D / 32; ++w)
+          ldmatrix_x4_trans(r[w], base + h * C::TILE + 16 * D + tile_offset<D>(m_row, 2 * w + m_piece));
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const uint32_t y0 = r[2 * half] ^ 0x80808080u, y1 = r[2 * half + 1] ^ 0x80808080u;
+            const uint32_t y0 = r[w][2 * half] ^ 0x80808080u, y1 = r[w][2 * half + 1] ^ 0x80808080u;
             const uint32_t va[4] = {widen(y0, 0x4240u), widen(y0, 0x4341u), widen(y1, 0x4240u), widen(y1, 0x4341u)};
 #pragma unroll
             for (int ng = 0; ng < NG; ++ng) mma_f16_16816(o[ng][2 * w + half], va, pb[ng][h][0], pb[ng][h][1]);
           }
-        }
+      }
       __syncwarp();
     }
 
@@ -617,7 +653,7 @@ PagedArgs args_of(const sl8_paged_cache& c, const sl8_paged_attn_params& p) {
 
 Plan plan_of(const PagedArgs& a, int D) {
   Plan x{};
-  x.ng = a.rows <= 8 ? 1 : (a.rows <= 16 ? 2 : groups_of(D));
+  x.ng = (int)std::min<int64_t>(groups_of(D), (a.rows + 7) / 8);
   x.row_warps = a.rows > 8 * groups_of(D) ? 2 : 1;   // PaCfg::ROW_WARPS
   x.rows_per_unit = x.row_warps * x.ng * 8;
   x.row_units = (a.rows + x.rows_per_unit - 1) / x.rows_per_unit;
@@ -670,6 +706,9 @@ int launch_paged_rows(const PagedArgs& a, int ng, cudaStream_t stream) {
   switch (ng) {
     case 1: return launch_paged<D, 1>(a, stream);
     case 2: return launch_paged<D, 2>(a, stream);
+    case 3:
+      if constexpr (D == 256) return SL8_ERR_UNSUPPORTED;
+      else return launch_paged<D, 3>(a, stream);
     default:
       if constexpr (D == 256) return SL8_ERR_UNSUPPORTED;
       else return launch_paged<D, 4>(a, stream);
