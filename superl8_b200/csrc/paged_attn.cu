@@ -65,6 +65,21 @@ __device__ Line line_of(const PagedArgs& a, int units, unsigned* red) {
   return l;
 }
 
+// The unit and the chunk in it that lie at place c of the line (every c < total is found by one thread).
+__device__ void locate(const PagedArgs& a, const Line& line, int units, unsigned c, int (&found)[3]) {
+  unsigned at = line.begin;
+  if (at > c) return;
+  for (int b = line.b0; b < line.b1; ++b) {
+    const unsigned chunks = seq_of(a, b).chunks, own = chunks * units;
+    if (c >= at && c - at < own) {
+      found[0] = b;
+      found[1] = (int)((c - at) / chunks);
+      found[2] = (int)((c - at) % chunks);
+    }
+    at += own;
+  }
+}
+
 // Chunks per block: equal shares, whole rounds of the block's warps.
 __device__ __forceinline__ unsigned share_of(unsigned total, int blocks) {
   const unsigned per = (total + blocks - 1) / blocks;
@@ -132,11 +147,46 @@ struct PaCfg {
   static_assert(smem(ROW_WARPS) <= 226 * 1024, "over the shared memory of an SM");
 };
 
+// Four channels of output row r of a unit: sum / l, zeros where the row has no query or saw no key.
+__device__ __forceinline__ void store_row(const PagedArgs& a, int b, int hkv, int r, int n, int ch, float4 sum, float l) {
+  const int i = r / a.G, head = hkv * a.G + r - i * a.G;
+  const float inv = (i < n && l != 0.f) ? 1.f / l : 0.f;
+  if (inv == 0.f) sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  uint2 y;
+  if (a.bf16) y = make_uint2(pack2<__nv_bfloat16>(sum.x * inv, sum.y * inv), pack2<__nv_bfloat16>(sum.z * inv, sum.w * inv));
+  else y = make_uint2(pack2<__half>(sum.x * inv, sum.y * inv), pack2<__half>(sum.z * inv, sum.w * inv));
+  *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + b * a.o_sb + head * a.o_sh + i * a.o_ss + ch) = y;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, int rank) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+  return at;
+}
+__device__ __forceinline__ float2 cluster_load2(const float2* p, int rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(cluster_addr(p, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 cluster_load4(const float* p, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(cluster_addr(p, rank))
+               : "memory");
+  return v;
+}
+
 // A row's reference M moves only when a logit passes it by this much (in powers of two): the weights stay
 // below 2^8, far inside fp16, and the accumulators are hardly ever rescaled.
 constexpr float kSlack = 8.f;
 
-template <int D, int NG>
+// CLUSTER: the blocks of a thread-block cluster share one unit and join through distributed shared memory,
+// so no second kernel follows; otherwise the block takes its range of the line.
+template <int D, int NG, bool CLUSTER>
 __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedArgs a) {
   using C = PaCfg<D, NG>;
   constexpr int T = C::TILES, KEYS = 1 << C::SHIFT;
@@ -148,31 +198,11 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
   uint4* qf = reinterpret_cast<uint4*>(smem + C::RING + C::BUF + C::ML); // [group][D / 32][lane]
   float* qs = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(qf) + a.row_warps * NG * C::Q_GROUP);
 
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if constexpr (!CLUSTER) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int key_warps = kPaWarps / a.row_warps;
   const int rw = warp / key_warps, kw = warp - rw * key_warps;
   const int units = a.Hkv * a.row_units;                                 // of one sequence
-
-  // ---- this block's range of the line ----
-  const Line line = line_of(a, units, red);
-  const unsigned per = share_of(line.total, a.blocks);
-  const unsigned c0 = min(line.total, per * blockIdx.x);
-  const unsigned c1 = min(line.total, c0 + per);
-  if (c0 >= c1) return;
-  if (line.begin <= c0) {
-    unsigned at = line.begin;
-    for (int b = line.b0; b < line.b1; ++b) {
-      const unsigned chunks = seq_of(a, b).chunks, own = chunks * units;
-      if (c0 >= at && c0 - at < own) {
-        s_start[0] = b;
-        s_start[1] = (int)((c0 - at) / chunks);
-        s_start[2] = (int)((c0 - at) % chunks);
-      }
-      at += own;
-    }
-  }
-  __syncthreads();
 
   // ---- the two cursors of a warp: compute, and the loads that run ahead of it across units ----
   struct Cursor {
@@ -193,10 +223,29 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
     open(x, 0);
   };
   Cursor cur;
-  cur.b = s_start[0]; cur.u = s_start[1];
-  cur.s = seq_of(a, cur.b);
-  cur.left = (int)(c1 - c0);
-  int c_begin = s_start[2];
+  int c_begin;
+  if constexpr (CLUSTER) {
+    // equal shares of the unit; a block without one still joins
+    const int unit = blockIdx.x / a.blocks, rank = blockIdx.x - unit * a.blocks;
+    cur.b = unit / units;
+    cur.u = unit - cur.b * units;
+    cur.s = seq_of(a, cur.b);
+    const int per = (cur.s.chunks + a.blocks - 1) / a.blocks;
+    c_begin = min(cur.s.chunks, rank * per);
+    cur.left = min(per, cur.s.chunks - c_begin);
+  } else {
+    const Line line = line_of(a, units, red);
+    const unsigned per = share_of(line.total, a.blocks);
+    const unsigned c0 = min(line.total, per * blockIdx.x);
+    const unsigned c1 = min(line.total, c0 + per);
+    if (c0 >= c1) return;
+    locate(a, line, units, c0, s_start);
+    __syncthreads();
+    cur.b = s_start[0]; cur.u = s_start[1];
+    cur.s = seq_of(a, cur.b);
+    cur.left = (int)(c1 - c0);
+    c_begin = s_start[2];
+  }
   open(cur, c_begin);
 
   uint8_t* ring = smem + warp * C::STAGES * C::SLOT;
@@ -498,8 +547,11 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
         l += __shfl_xor_sync(0xffffffffu, l, 16);
         if (g == 0) ml[warp * NG * 8 + ng * 8 + 2 * t + e] = make_float2(m_run[ng][e], l);
       }
+    if constexpr (CLUSTER) cp_async_wait<0>();      // the ring becomes the cluster's partials
     __syncthreads();
-    const bool complete = c_begin == 0 && cur.cend == s.chunks;
+    const bool complete = !CLUSTER && c_begin == 0 && cur.cend == s.chunks;
+    float* const res_o = reinterpret_cast<float*>(smem);                 // [rows_per_unit][D]
+    float2* const res_ml = reinterpret_cast<float2*>(res_o + a.rows_per_unit * D);
     const int64_t part = (2ll * blockIdx.x + (c_begin == 0)) * a.rows_per_unit;
     const float2* my_ml = ml + rw * key_warps * NG * 8;
 #pragma unroll
@@ -533,16 +585,11 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
             sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
           }
           const int r_local = (rw * NG + ng) * 8 + row, r = row0 + r_local;
-          if (complete) {
-            if (r < a.rows) {
-              const int i = r / a.G, head = hkv * a.G + r % a.G;
-              const float inv = (i < s.n && l != 0.f) ? 1.f / l : 0.f;
-              if (inv == 0.f) sum = make_float4(0.f, 0.f, 0.f, 0.f);
-              uint2 y;
-              if (a.bf16) y = make_uint2(pack2<__nv_bfloat16>(sum.x * inv, sum.y * inv), pack2<__nv_bfloat16>(sum.z * inv, sum.w * inv));
-              else y = make_uint2(pack2<__half>(sum.x * inv, sum.y * inv), pack2<__half>(sum.z * inv, sum.w * inv));
-              *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + cur.b * a.o_sb + head * a.o_sh + i * a.o_ss + d0 + ch) = y;
-            }
+          if constexpr (CLUSTER) {
+            *reinterpret_cast<float4*>(res_o + r_local * D + d0 + ch) = sum;
+            if (d0 + ch == 0) res_ml[r_local] = make_float2(m, l);
+          } else if (complete) {
+            if (r < a.rows) store_row(a, cur.b, hkv, r, s.n, d0 + ch, sum, l);
           } else {
             *reinterpret_cast<float4*>(a.part_o + (part + r_local) * D + d0 + ch) = sum;
             if (d0 + ch == 0) *reinterpret_cast<float2*>(a.part_ml + (part + r_local) * 2) = make_float2(m, l);
@@ -551,70 +598,110 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
         __syncthreads();
       }
     }
-    if (cur.left <= 0) break;
-    next_unit(cur);
-    c_begin = 0;
+    if constexpr (CLUSTER) {
+      cluster_sync();
+      const int rank = blockIdx.x % a.blocks;
+      for (int idx = rank * kPaThreads + tid; idx < a.rows_per_unit * (D / 4); idx += a.blocks * kPaThreads) {
+        const int r_local = idx / (D / 4), ch = idx % (D / 4) * 4, r = row0 + r_local;
+        if (r >= a.rows) break;
+        float m = kNegSentinel, l = 0.f;
+        for (int c = 0; c < a.blocks; ++c) m = fmaxf(m, cluster_load2(res_ml + r_local, c).x);
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = 0; c < a.blocks; ++c) {
+          const float2 one = cluster_load2(res_ml + r_local, c);
+          const float f = ex2_approx(one.x - m);
+          const float4 x = cluster_load4(res_o + r_local * D + ch, c);
+          l = fmaf(one.y, f, l);
+          sum.x = fmaf(x.x, f, sum.x); sum.y = fmaf(x.y, f, sum.y); sum.z = fmaf(x.z, f, sum.z); sum.w = fmaf(x.w, f, sum.w);
+        }
+        store_row(a, cur.b, hkv, r, s.n, ch, sum, l);
+      }
+      cluster_sync();   // a block's shared memory outlives its readers
+      break;
+    } else {
+      if (cur.left <= 0) break;
+      next_unit(cur);
+      c_begin = 0;
+    }
   }
   cp_async_wait<0>();
 }
 
-// Joins the partials of the units that more than one block worked on, and writes the zeros of sequences
-// without keys or queries.  One block per unit, one warp per row at a time.
+// Behind the split kernel, with its grid: block i joins the partials of the unit that begins in range i and ends
+// behind it (at most one), a warp per row, and writes the zeros of every sequence without keys or queries.
 template <int D>
-__global__ void __launch_bounds__(kPaThreads) paged_join_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(kPaThreads, 1) paged_join_kernel(const PagedArgs a) {
   __shared__ unsigned red[kPaWarps];
-  __shared__ unsigned s_before;
+  __shared__ int s_last[3];
   const int units = a.Hkv * a.row_units;
-  const int b = blockIdx.x / units, u = blockIdx.x - b * units;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Line line = line_of(a, units, red);
-  if (line.b0 <= b && b < line.b1) {               // the chunks of the sequences before b
-    unsigned at = line.begin;
-    for (int j = line.b0; j < b; ++j) at += seq_of(a, j).chunks * units;
-    s_before = at;
-  }
-  __syncthreads();
-  const Seq s = seq_of(a, b);
   const unsigned per = share_of(line.total, a.blocks);
-  const unsigned g0 = s_before + (unsigned)u * s.chunks;
-  const unsigned i0 = g0 / per, i1 = s.chunks > 0 ? (g0 + s.chunks - 1) / per : i0;
+  const unsigned c0 = min(line.total, per * blockIdx.x), c1 = min(line.total, c0 + per);
+  if (c0 < c1) locate(a, line, units, c1 - 1, s_last);
+  __syncthreads();
+  for (int b = blockIdx.x; b < a.B; b += a.blocks) {
+    if (seq_of(a, b).chunks > 0) continue;
+    for (int64_t idx = threadIdx.x; idx < (int64_t)a.Hq * a.M * (D / 4); idx += kPaThreads) {
+      const int ch = (int)(idx % (D / 4)) * 4, head = (int)(idx / (D / 4) % a.Hq), i = (int)(idx / (D / 4) / a.Hq);
+      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + b * a.o_sb + head * a.o_sh + i * a.o_ss + ch) = make_uint2(0, 0);
+    }
+  }
   // every block waits, also one with nothing to do: a grid that ended before the split kernel would let
   // the stream's next kernel start beside it
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (s.chunks > 0 && i0 == i1) return;            // finished by its block
-  const int hkv = u / a.row_units, row0 = (u % a.row_units) * a.rows_per_unit;
-  constexpr int PER = D / 32;                       // channels per lane
+  if (c0 >= c1) return;
+  const int b = s_last[0], u = s_last[1];
+  const Seq s = seq_of(a, b);
+  const unsigned back = s_last[2];                            // chunks of the unit before c1 - 1
+  if (back > c1 - 1 - c0 || (int)back == s.chunks - 1) return;   // it began in an earlier range, or ends in this one
+  const unsigned i0 = blockIdx.x, i1 = (c1 - 1 - back + s.chunks - 1) / per;
+  const int hkv = u / a.row_units, row0 = (u - hkv * a.row_units) * a.rows_per_unit;
+  const int parts = (int)(i1 - i0 + 1);
+  constexpr int PER = D >= 128 ? 4 : D / 32;                  // channels per lane and pass
   for (int r_local = warp; r_local < a.rows_per_unit && row0 + r_local < a.rows; r_local += kPaWarps) {
-    const int r = row0 + r_local, i = r / a.G, head = hkv * a.G + r % a.G;
-    float sum[PER];
+    const int r = row0 + r_local;
+    // partial n: block i0 + n, its slot 1 where it began the unit (n = 0), else slot 0
+    auto row_of = [&](int n) { return (int64_t)(2 * (i0 + n) + (n == 0)) * a.rows_per_unit + r_local; };
+    float m = kNegSentinel;
+    for (int n = lane; n < parts; n += 32) m = fmaxf(m, a.part_ml[row_of(n) * 2]);
 #pragma unroll
-    for (int e = 0; e < PER; ++e) sum[e] = 0.f;
-    float l = 0.f;
-    if (s.chunks > 0 && i < s.n) {
-      // partial n: block i0 + n, its slot 1 where it began the unit (n = 0), else slot 0
-      float m = kNegSentinel;
-      const int parts = (int)(i1 - i0 + 1);
-      auto row_of = [&](int n) { return (int64_t)(2 * (i0 + n) + (n == 0)) * a.rows_per_unit + r_local; };
-      for (int n = lane; n < parts; n += 32) m = fmaxf(m, a.part_ml[row_of(n) * 2]);
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
 #pragma unroll
-      for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-#pragma unroll 4
+    for (int d0 = 0; d0 < D; d0 += 32 * PER) {
+      float sum[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+#pragma unroll 8
       for (int n = 0; n < parts; ++n) {
         const float2 one = *reinterpret_cast<const float2*>(a.part_ml + row_of(n) * 2);
+        const float* src = a.part_o + row_of(n) * D + d0 + PER * lane;
+        float x[4];
+        if constexpr (PER == 4) {
+          const float4 v = *reinterpret_cast<const float4*>(src);
+          x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+        } else if constexpr (PER == 2) {
+          const float2 v = *reinterpret_cast<const float2*>(src);
+          x[0] = v.x; x[1] = v.y;
+        } else {
+          x[0] = *src;
+        }
         const float f = ex2_approx(one.x - m);
         l = fmaf(one.y, f, l);
-        const float* src = a.part_o + row_of(n) * D + PER * lane;
 #pragma unroll
-        for (int e = 0; e < PER; ++e) sum[e] = fmaf(src[e], f, sum[e]);
+        for (int e = 0; e < PER; ++e) sum[e] = fmaf(x[e], f, sum[e]);
       }
-    }
-    const float inv = l != 0.f ? 1.f / l : 0.f;
-    uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + b * a.o_sb + head * a.o_sh + i * a.o_ss + PER * lane;
+      if constexpr (PER == 4) {
+        store_row(a, b, hkv, r, s.n, d0 + 4 * lane, make_float4(sum[0], sum[1], sum[2], sum[3]), l);
+      } else {
+        // four channels from the neighbouring lanes
+        float y[4];
 #pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      const float y = inv == 0.f ? 0.f : sum[e] * inv;
-      if (a.bf16) reinterpret_cast<__nv_bfloat16*>(dst)[e] = __float2bfloat16_rn(y);
-      else reinterpret_cast<__half*>(dst)[e] = __float2half_rn(y);
+        for (int e = 0; e < 4; ++e) {
+          const float z0 = __shfl_sync(0xffffffffu, sum[0], (4 * lane + e) / PER & 31);
+          const float z1 = __shfl_sync(0xffffffffu, sum[PER - 1], (4 * lane + e) / PER & 31);
+          y[e] = PER == 1 || e % 2 == 0 ? z0 : z1;
+        }
+        if (lane < D / 4) store_row(a, b, hkv, r, s.n, 4 * lane, make_float4(y[0], y[1], y[2], y[3]), l);
+      }
     }
   }
 }
@@ -622,7 +709,9 @@ __global__ void __launch_bounds__(kPaThreads) paged_join_kernel(const PagedArgs 
 // Rows that one unit of the split kernel serves: 8 per group of the MMA's N axis, groups per warp (NG), warps
 // with other rows.
 struct Plan {
-  int ng, row_warps, row_units, rows_per_unit, blocks;
+  int ng, row_warps, row_units, rows_per_unit;
+  bool cluster;           // blocks = blocks per unit, else of the whole grid
+  int blocks;
   size_t prefill_bytes;   // > 0: paged_prefill.cu serves the call, with this workspace
 };
 
@@ -634,6 +723,11 @@ int page_shift_of(int page_size) {
     if (page_size == (1 << s)) return s;
   return -1;
 }
+
+int key_warps_of(const Plan& x) { return kPaWarps / x.row_warps; }
+
+// Chunks per warp up to which a cluster per unit is used.
+constexpr int kClusterSteps = 4;
 
 PagedArgs args_of(const sl8_paged_cache& c, const sl8_paged_attn_params& p) {
   PagedArgs a{};
@@ -661,6 +755,16 @@ Plan plan_of(const PagedArgs& a, int D) {
   const int64_t chunks = ((int64_t)a.max_tokens + keys - 1) / keys * a.B * a.Hkv * x.row_units;
   const int64_t want = (chunks + kPaWarps - 1) / kPaWarps;
   x.blocks = (int)(want < 1 ? 1 : (want > kNumSms ? kNumSms : want));
+  // Few units of few chunks: a cluster per unit, up to eight blocks with a chunk per warp at least, as long as
+  // that is at most kClusterSteps chunks per warp and all clusters run at once (of eight blocks, sixteen do).
+  const int64_t units = (int64_t)a.B * a.Hkv * x.row_units, longest = ((int64_t)a.max_tokens + keys - 1) / keys;
+  int per_unit = 1;
+  while (per_unit < 8 && units * per_unit * 2 <= 128 && (int64_t)per_unit * kPaWarps < longest) per_unit *= 2;
+  const int64_t steps = (longest + (int64_t)per_unit * key_warps_of(x) - 1) / ((int64_t)per_unit * key_warps_of(x));
+  if (units * per_unit <= kNumSms && steps <= kClusterSteps) {
+    x.cluster = true;
+    x.blocks = per_unit;
+  }
   x.prefill_bytes = a.rows >= kPrefillRows ? sl8_paged_prefill_workspace(a, D) : 0;
   return x;
 }
@@ -675,43 +779,60 @@ int paged_checks(const sl8_paged_cache* c, const sl8_paged_attn_params* p) {
   return SL8_OK;
 }
 
-template <int D, int NG>
-int launch_paged(const PagedArgs& a, cudaStream_t stream) {
+template <int D, int NG, bool CLUSTER>
+int allow_smem() {
   static std::atomic<bool> allowed[64];
   int dev = 0;
   SL8_CUDA_TRY(cudaGetDevice(&dev));
-  if (dev >= 64 || !allowed[dev].load()) {
-    SL8_CUDA_TRY(cudaFuncSetAttribute(paged_split_kernel<D, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      PaCfg<D, NG>::smem(PaCfg<D, NG>::ROW_WARPS)));
-    if (dev < 64) allowed[dev].store(true);
-  }
+  if (dev < 64 && allowed[dev].load()) return SL8_OK;
+  SL8_CUDA_TRY(cudaFuncSetAttribute(paged_split_kernel<D, NG, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    PaCfg<D, NG>::smem(PaCfg<D, NG>::ROW_WARPS)));
+  if (dev < 64) allowed[dev].store(true);
+  return SL8_OK;
+}
+
+template <int D, int NG>
+int launch_paged(const PagedArgs& a, bool cluster, cudaStream_t stream) {
   const int smem = PaCfg<D, NG>::smem(a.row_warps);
-  paged_split_kernel<D, NG><<<a.blocks, kPaThreads, smem, stream>>>(a);
-  if (cudaGetLastError() != cudaSuccess) return SL8_ERR_CUDA;
   cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute early{};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)(a.B * a.Hkv * a.row_units));
+  cudaLaunchAttribute attr{};
   cfg.blockDim = dim3(kPaThreads);
   cfg.stream = stream;
-  cfg.attrs = &early;
+  cfg.attrs = &attr;
   cfg.numAttrs = 1;
+  if (cluster) {
+    const int rc = allow_smem<D, NG, true>();
+    if (rc != SL8_OK) return rc;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)a.blocks;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)(a.B * a.Hkv * a.row_units * a.blocks));
+    cfg.dynamicSmemBytes = smem;
+    SL8_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_split_kernel<D, NG, true>, a));
+    return SL8_OK;
+  }
+  const int rc = allow_smem<D, NG, false>();
+  if (rc != SL8_OK) return rc;
+  paged_split_kernel<D, NG, false><<<a.blocks, kPaThreads, smem, stream>>>(a);
+  if (cudaGetLastError() != cudaSuccess) return SL8_ERR_CUDA;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)a.blocks);
   SL8_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_join_kernel<D>, a));
   return SL8_OK;
 }
 
 template <int D>
-int launch_paged_rows(const PagedArgs& a, int ng, cudaStream_t stream) {
+int launch_paged_rows(const PagedArgs& a, int ng, bool cluster, cudaStream_t stream) {
   switch (ng) {
-    case 1: return launch_paged<D, 1>(a, stream);
-    case 2: return launch_paged<D, 2>(a, stream);
+    case 1: return launch_paged<D, 1>(a, cluster, stream);
+    case 2: return launch_paged<D, 2>(a, cluster, stream);
     case 3:
       if constexpr (D == 256) return SL8_ERR_UNSUPPORTED;
-      else return launch_paged<D, 3>(a, stream);
+      else return launch_paged<D, 3>(a, cluster, stream);
     default:
       if constexpr (D == 256) return SL8_ERR_UNSUPPORTED;
-      else return launch_paged<D, 4>(a, stream);
+      else return launch_paged<D, 4>(a, cluster, stream);
   }
 }
 
@@ -724,6 +845,7 @@ extern "C" size_t sl8_attn_paged_workspace(const sl8_paged_cache* c, const sl8_p
   if (paged_checks(c, p) != SL8_OK || (int64_t)p->B * p->Hq * p->M == 0) return 1024;
   const Plan x = plan_of(args_of(*c, *p), c->D);
   if (x.prefill_bytes > 0) return 1024 + x.prefill_bytes;
+  if (x.cluster) return 1024;
   return 1024 + (size_t)2 * x.blocks * x.rows_per_unit * (c->D + 2) * sizeof(float);
 }
 
@@ -754,9 +876,9 @@ extern "C" int sl8_attn_paged(const sl8_paged_cache* c, const sl8_paged_attn_par
   a.part_ml = a.part_o + (size_t)2 * x.blocks * x.rows_per_unit * c->D;
   a.row_warps = x.row_warps; a.rows_per_unit = x.rows_per_unit; a.row_units = x.row_units; a.blocks = x.blocks;
   switch (c->D) {
-    case 32: return launch_paged_rows<32>(a, x.ng, s);
-    case 64: return launch_paged_rows<64>(a, x.ng, s);
-    case 128: return launch_paged_rows<128>(a, x.ng, s);
-    default: return launch_paged_rows<256>(a, x.ng, s);
+    case 32: return launch_paged_rows<32>(a, x.ng, x.cluster, s);
+    case 64: return launch_paged_rows<64>(a, x.ng, x.cluster, s);
+    case 128: return launch_paged_rows<128>(a, x.ng, x.cluster, s);
+    default: return launch_paged_rows<256>(a, x.ng, x.cluster, s);
   }
 }

@@ -351,6 +351,26 @@ def test_attend_sees_no_key_past_the_stated_length(device, M):
         held_to(s8.attn_paged_cached(*args, max_context_len=limit), q, cache, table, lens, limit=limit)
 
 
+# More units than SMs, or more chunks than a cluster takes: the line of all units is cut into equal ranges
+LINE = [
+    ([7, 0, 33, 64, 100, 1] * 16, 4, 2, 1, 64, 16, torch.float16, True, -1, None),
+    ([300, 5, 0, 170] * 10, 10, 5, 1, 128, 32, torch.bfloat16, True, 37, None),
+    ([65, 130, 31] * 14, 20, 4, 4, 128, 16, torch.float16, True, -1, [4, 2, 0] * 14),
+    ([90, 40] * 45, 6, 2, 9, 64, 64, torch.bfloat16, True, -1, None),
+    ([20, 70] * 40, 4, 2, 20, 32, 16, torch.float16, False, -1, None),
+    ([33, 48] * 45, 4, 2, 3, 256, 16, torch.float16, True, -1, None),
+    ([129] * 80, 16, 2, 5, 256, 64, torch.float16, True, 60, None),
+    ([21000], 4, 1, 1, 128, 64, torch.float16, True, -1, None),
+    ([9000, 17], 8, 1, 6, 64, 128, torch.bfloat16, True, -1, [6, 6]),
+    ([9000], 2, 1, 1, 32, 256, torch.float16, True, -1, None),
+]
+
+
+@pytest.mark.parametrize("case", LINE)
+def test_many_units_against_definition(device, case):
+    attend_case(device, case)
+
+
 PREFILL = [  # lens, Hq, Hkv, M, D, page, dtype, causal, window, query_lens
     ([200], 4, 4, 200, 128, 16, torch.float16, True, -1, None),
     ([300, 77, 0, 129], 8, 2, 77, 128, 64, torch.bfloat16, True, -1, [77, 77, 0, 40]),
