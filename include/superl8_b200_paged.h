@@ -120,7 +120,7 @@ size_t sl8_attn_paged_workspace(const sl8_paged_cache* cache, const sl8_paged_at
 int sl8_attn_paged(const sl8_paged_cache* cache, const sl8_paged_attn_params* p, void* workspace,
                    size_t workspace_bytes, void* stream);
 
-/* Synchronises the stream and returns the status of the tensor-memory kernel's bounded waits on the current
+/* Synchronises the stream and returns the status of these kernels' bounded waits on the current
  * device since the last call (SL8_OK or SL8_ERR_DEVICE_TIMEOUT), and clears it. */
 int sl8_paged_status(void* stream);
 

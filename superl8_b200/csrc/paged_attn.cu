@@ -13,7 +13,7 @@
 // times the query tokens) are served by one pass over its keys, with keys on the M axis of the MMA (tiles
 // of 16) and 8 query rows on the N axis, so a group of 8 heads wastes nothing.  Every warp streams
 // its own chunks of 32 or 16 keys (a 16-key tile never crosses a page: page sizes are multiples of 16) through
-// a private ring of cp.async stages: no barrier inside the loop, 128 KB in flight per SM.
+// a private ring of TMA stages: no barrier between warps inside the loop, 128 KB in flight per SM.
 //
 // Split.  The chunks of all (sequence, KV head) units form one line, cut into equal ranges, one per block
 // of a one-block-per-SM grid, whatever the lengths are; a unit that lies in one range is finished there,
@@ -27,6 +27,8 @@
 
 namespace sl8 {
 namespace {
+
+__device__ int g_paged_wait_status;   // raised by an expired wait; zero when the library is loaded
 
 constexpr int kPaWarps = 8;
 constexpr int kPaThreads = 32 * kPaWarps;
@@ -66,7 +68,7 @@ __device__ Line line_of(const PagedArgs& a, int units, unsigned* red) {
 }
 
 // The unit and the chunk in it that lie at place c of the line (every c < total is found by one thread).
-__device__ void locate(const PagedArgs& a, const Line& line, int units, unsigned c, int (&found)[3]) {
+__device__ __forceinline__ void locate(const PagedArgs& a, const Line& line, int units, unsigned c, int (&found)[3]) {
   unsigned at = line.begin;
   if (at > c) return;
   for (int b = line.b0; b < line.b1; ++b) {
@@ -81,26 +83,11 @@ __device__ void locate(const PagedArgs& a, const Line& line, int units, unsigned
 }
 
 // Chunks per block: equal shares, whole rounds of the block's warps.
-__device__ __forceinline__ unsigned share_of(unsigned total, int blocks) {
-  const unsigned per = (total + blocks - 1) / blocks;
+__device__ __forceinline__ unsigned share_of(const PagedArgs& a, unsigned total) {
+  const unsigned per = (total + a.blocks - 1) / a.blocks;
   return max((unsigned)kPaWarps, (per + kPaWarps - 1) / kPaWarps * kPaWarps);
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
-  uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
-}
 __device__ __forceinline__ float lg2_approx(float x) {
   float y;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -112,18 +99,22 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return y;
 }
 
-// 16-byte piece `c` of row `r` of a [16][D] byte tile: pieces are exchanged within 128 bytes so that the
-// eight rows of an ldmatrix lie in eight different bank groups.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// Where 16-byte piece `c` of row `r` of a 16-key tile lies in shared memory: sub-tiles of at most 128 bytes a
+// row, as the copy engine's swizzle leaves them (the eight rows of an ldmatrix in eight different bank groups).
 template <int D>
 __device__ __forceinline__ uint32_t tile_offset(int r, int c) {
-  constexpr int SH = D >= 128 ? 0 : (D == 64 ? 1 : 2);
-  constexpr int MASK = D >= 128 ? 7 : D / 16 - 1;
-  return r * D + ((c ^ ((r >> SH) & MASK)) << 4);
+  constexpr int ROW = D < 128 ? D : 128, SW = D >= 128 ? 3 : (D == 64 ? 2 : 1);
+  return (c / (ROW / 16)) * (16 * ROW) + swizzle_offset<SW>(r * ROW + (c % (ROW / 16)) * 16);
 }
 
 // Keys per warp and step: 32 (two 16-key tiles share the maximum, the rescaling and the loop) where the
 // accumulators leave the registers for it and the ring the space, else 16.
-__host__ __device__ constexpr int chunk_shift_of(int D, int ng) { return D == 256 || (D >= 64 && ng >= 3) ? 4 : 5; }
+__host__ __device__ constexpr int chunk_shift_of(int D, int ng) { return D == 256 || (D == 128 && ng == 4) ? 4 : 5; }
 
 // Most groups of 8 query rows a warp can accumulate: D / 4 registers a thread each.
 __host__ __device__ constexpr int groups_of(int D) { return D == 256 ? 2 : 4; }
@@ -132,31 +123,22 @@ template <int D, int NG>
 struct PaCfg {
   static constexpr int SHIFT = chunk_shift_of(D, NG);
   static constexpr int TILES = (1 << SHIFT) / 16;                        // 16-key tiles per chunk
-  static constexpr int TILE = 2 * 16 * D + 16;                           // K rows, V rows, the two scales
+  static constexpr int TILE = 2 * 16 * D;                                // K rows, V rows
   static constexpr int SLOT = TILES * TILE;
-  static constexpr int STAGES = D == 256 ? 2 : (D == 128 ? (TILES == 2 ? 3 : 5) : (D == 64 ? (TILES == 2 ? 5 : 10) : 8));
+  static constexpr int SUBS = D <= 128 ? 1 : D / 128, ROW = D / SUBS;    // sub-tiles of at most 128 bytes a row
+  static constexpr int STAGES = D == 256 ? 2 : (D == 128 ? (TILES == 2 ? 3 : 5) : (D == 64 ? 5 : 8));
   static constexpr int RING = kPaWarps * STAGES * SLOT;
+  static constexpr int SIDE = kPaWarps * STAGES * (TILES * 8 + 8);       // the tiles' scales, the slots' barriers
   static constexpr int JOIN = D >= 128 ? D / 2 : D;                      // channels joined at a time
   static constexpr int BUF_ROW = JOIN + 8;                               // floats per row of the joining buffer
   static constexpr int BUF = kPaWarps * 8 * BUF_ROW * 4;
   static constexpr int Q_GROUP = D * 16;                                 // two int8 planes of 8 rows, fragment order
-  static constexpr int ML = kPaWarps * NG * 8 * 8;
   static constexpr int ROW_WARPS = NG == groups_of(D) ? 2 : 1;           // most warps with rows of their own
+  static constexpr int ML = (kPaWarps + ROW_WARPS) * NG * 8 * 8;         // per warp and row, and per row
   static constexpr bool Q_REGS = NG * D <= 256;                          // fragments of Q held in registers
-  static constexpr int smem(int row_warps) { return RING + BUF + ML + row_warps * NG * (Q_GROUP + 32); }
+  static constexpr int smem(int row_warps) { return 1024 + RING + SIDE + BUF + ML + row_warps * NG * (Q_GROUP + 32); }
   static_assert(smem(ROW_WARPS) <= 226 * 1024, "over the shared memory of an SM");
 };
-
-// Four channels of output row r of a unit: sum / l, zeros where the row has no query or saw no key.
-__device__ __forceinline__ void store_row(const PagedArgs& a, int b, int hkv, int r, int n, int ch, float4 sum, float l) {
-  const int i = r / a.G, head = hkv * a.G + r - i * a.G;
-  const float inv = (i < n && l != 0.f) ? 1.f / l : 0.f;
-  if (inv == 0.f) sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  uint2 y;
-  if (a.bf16) y = make_uint2(pack2<__nv_bfloat16>(sum.x * inv, sum.y * inv), pack2<__nv_bfloat16>(sum.z * inv, sum.w * inv));
-  else y = make_uint2(pack2<__half>(sum.x * inv, sum.y * inv), pack2<__half>(sum.z * inv, sum.w * inv));
-  *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + b * a.o_sb + head * a.o_sh + i * a.o_ss + ch) = y;
-}
 
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
@@ -180,6 +162,17 @@ __device__ __forceinline__ float4 cluster_load4(const float* p, int rank) {
   return v;
 }
 
+// Four channels of output row r of a unit: sum / l, zeros where the row has no query or saw no key.
+__device__ __forceinline__ void store_row(const PagedArgs& a, int b, int hkv, int r, int n, int ch, float4 sum, float l) {
+  const int i = r / a.G, head = hkv * a.G + r - i * a.G;
+  const float inv = (i < n && l != 0.f) ? 1.f / l : 0.f;
+  if (inv == 0.f) sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  uint2 y;
+  if (a.bf16) y = make_uint2(pack2<__nv_bfloat16>(sum.x * inv, sum.y * inv), pack2<__nv_bfloat16>(sum.z * inv, sum.w * inv));
+  else y = make_uint2(pack2<__half>(sum.x * inv, sum.y * inv), pack2<__half>(sum.z * inv, sum.w * inv));
+  *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + b * a.o_sb + head * a.o_sh + i * a.o_ss + ch) = y;
+}
+
 // A row's reference M moves only when a logit passes it by this much (in powers of two): the weights stay
 // below 2^8, far inside fp16, and the accumulators are hardly ever rescaled.
 constexpr float kSlack = 8.f;
@@ -187,15 +180,20 @@ constexpr float kSlack = 8.f;
 // CLUSTER: the blocks of a thread-block cluster share one unit and join through distributed shared memory,
 // so no second kernel follows; otherwise the block takes its range of the line.
 template <int D, int NG, bool CLUSTER>
-__global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const __grid_constant__ CUtensorMap k_map,
+                                                                    const __grid_constant__ CUtensorMap v_map,
+                                                                    const __grid_constant__ PagedArgs a) {
   using C = PaCfg<D, NG>;
   constexpr int T = C::TILES, KEYS = 1 << C::SHIFT;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ unsigned red[kPaWarps];
   __shared__ int s_start[3];
   float* buf = reinterpret_cast<float*>(smem + C::RING);
   float2* ml = reinterpret_cast<float2*>(smem + C::RING + C::BUF);       // [warp][NG * 8]
+  float2* joint = ml + kPaWarps * NG * 8;                                // [row_warps * NG * 8]: reference, sum
   uint4* qf = reinterpret_cast<uint4*>(smem + C::RING + C::BUF + C::ML); // [group][D / 32][lane]
+  float2* side = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(qf) + a.row_warps * NG * (C::Q_GROUP + 32));
   float* qs = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(qf) + a.row_warps * NG * C::Q_GROUP);
 
   if constexpr (!CLUSTER) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -203,6 +201,20 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
   const int key_warps = kPaWarps / a.row_warps;
   const int rw = warp / key_warps, kw = warp - rw * key_warps;
   const int units = a.Hkv * a.row_units;                                 // of one sequence
+  // this warp's ring, and beside it the scales of every tile and a barrier per slot
+  uint8_t* const ring = smem + warp * C::STAGES * C::SLOT;
+  float2* const scales_at = side + warp * C::STAGES * T;
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(side + kPaWarps * C::STAGES * T) + warp * C::STAGES;
+  if (lane == 0) {
+    if (warp == 0) {
+      tma_prefetch_desc(&k_map);
+      tma_prefetch_desc(&v_map);
+    }
+#pragma unroll
+    for (int i = 0; i < C::STAGES; ++i) mbar_init(&bars[i], T);
+    mbar_fence_init();
+  }
+  __syncwarp();
 
   // ---- the two cursors of a warp: compute, and the loads that run ahead of it across units ----
   struct Cursor {
@@ -235,7 +247,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
     cur.left = min(per, cur.s.chunks - c_begin);
   } else {
     const Line line = line_of(a, units, red);
-    const unsigned per = share_of(line.total, a.blocks);
+    const unsigned per = share_of(a, line.total);
     const unsigned c0 = min(line.total, per * blockIdx.x);
     const unsigned c1 = min(line.total, c0 + per);
     if (c0 >= c1) return;
@@ -248,12 +260,10 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
   }
   open(cur, c_begin);
 
-  uint8_t* ring = smem + warp * C::STAGES * C::SLOT;
-  const uint32_t ring_addr = smem_u32(ring);
-  // Loads of a chunk: a half-warp per tile when there are two (each tile has its own page), else the warp.
-  constexpr int LANES = 32 / T;                       // lanes that load one tile
-  const int l_tile = T == 2 ? lane >> 4 : 0, l_lane = lane & (LANES - 1);
-  const uint32_t l_dst = ring_addr + l_tile * C::TILE;
+  // Loads of a chunk: lane 16 h asks the copy engine for tile h (each tile has its own page) and carries its
+  // scales, which go to shared memory one step later.
+  const int l_tile = T == 2 ? lane >> 4 : 0;
+  const bool loader = (lane & 15) == 0 && lane < 16 * T;
   Cursor ahead = cur;
   const int32_t* a_row = a.table + ahead.b * a.table_stride;
   int a_head = ahead.u / a.row_units;
@@ -261,7 +271,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
   const int page_mask = (1 << a.page_shift) - 1;
   auto find_page = [&]() {   // the page of this lane's tile, asked for one step before it is needed
     a_tok = (ahead.s.first_chunk + ahead.c) * KEYS + 16 * l_tile;
-    page = a_tok < ahead.s.len ? __ldg(a_row + (a_tok >> a.page_shift)) : -1;
+    page = loader && a_tok < ahead.s.len ? __ldg(a_row + (a_tok >> a.page_shift)) : -1;
   };
   auto seek = [&]() {        // the next segment with a chunk for this warp; none: c stays at or past cend
     while (ahead.c >= ahead.cend && ahead.left > 0) {
@@ -272,34 +282,40 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
     if (ahead.c < ahead.cend) find_page();
   };
   seek();
+  float2 late = make_float2(0.f, 0.f);
+  int late_slot = -1;
   auto issue = [&](int slot) {
+    if (late_slot >= 0 && loader) scales_at[late_slot * T + l_tile] = late;
+    late_slot = -1;
     if (ahead.c < ahead.cend) {
-      const bool held = (unsigned)page < (unsigned)a.num_pages;   // otherwise zeros, and a scale of 0: nothing is seen
-      const int64_t ph = held ? (int64_t)page * a.Hkv + a_head : 0;
-      const int64_t at = held ? ((ph << a.page_shift) + (a_tok & page_mask)) * D + 16 * l_lane : 0;
-      const uint32_t dst = l_dst + slot * C::SLOT;
-      const int n16 = held ? 16 : 0;
-      const int8_t* ksrc = a.k + at;
-      const int8_t* vsrc = a.v + at;
+      late_slot = slot;
+      if (loader) {
+        late = make_float2(0.f, 0.f);                             // a missing page: scales of 0, nothing is seen
+        const bool held = (unsigned)page < (unsigned)a.num_pages;
+        if (held) {
+          const int ph = page * a.Hkv + a_head, row = a_tok & page_mask;
+          uint8_t* dst = ring + slot * C::SLOT + l_tile * C::TILE;
+          mbar_expect_tx(&bars[slot], C::TILE);
 #pragma unroll
-      for (int i = 0; i < D / LANES; ++i) {
-        const int idx = l_lane + LANES * i;
-        cp_async16(dst + tile_offset<D>(idx / (D / 16), idx % (D / 16)), ksrc + 16 * LANES * i, n16);
+          for (int i = 0; i < C::SUBS; ++i) {
+            tma_load_3d(dst + i * 16 * C::ROW, &k_map, &bars[slot], i * C::ROW, row, ph);
+            tma_load_3d(dst + 16 * D + i * 16 * C::ROW, &v_map, &bars[slot], i * C::ROW, row, ph);
+          }
+          late = make_float2(__ldg(a.ks + ph), __ldg(a.vs + ph));
+        } else {
+          mbar_arrive(&bars[slot]);
+        }
       }
-#pragma unroll
-      for (int i = 0; i < D / LANES; ++i) {
-        const int idx = l_lane + LANES * i;
-        cp_async16(dst + 16 * D + tile_offset<D>(idx / (D / 16), idx % (D / 16)), vsrc + 16 * LANES * i, n16);
-      }
-      if (l_lane < 2) cp_async4(dst + 32 * D + 4 * l_lane, (l_lane ? a.vs : a.ks) + ph, held ? 4 : 0);
       ahead.c += key_warps;
       if (ahead.c < ahead.cend) find_page(); else seek();
     }
-    cp_async_commit();
   };
 #pragma unroll 1
   for (int i = 0; i < C::STAGES - 1; ++i) issue(i);
   int slot_in = C::STAGES - 1, slot_out = 0;
+  uint32_t parity = 0;       // of slot_out's current use
+  bool ok = true;            // false once a bounded wait has expired: the block runs on without waiting
+  const uint32_t ring_addr = smem_u32(ring);
 
   // ldmatrix rows and pieces of this lane: K tiles [key][channel] and, transposing, V
   const int m_row = (lane & 7) + ((lane >> 3) & 1) * 8, m_piece = lane >> 4;
@@ -383,61 +399,67 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
     for (int c = cur.c; c < cur.cend; c += key_warps) {
       issue(slot_in);
       slot_in = slot_in + 1 == C::STAGES ? 0 : slot_in + 1;
-      cp_async_wait<C::STAGES - 1>();
+      if (ok) ok = mbar_wait(&bars[slot_out], parity, &g_paged_wait_status);
       __syncwarp();
       const uint32_t base = ring_addr + slot_out * C::SLOT;
-      const uint8_t* here = ring + slot_out * C::SLOT;
-      slot_out = slot_out + 1 == C::STAGES ? 0 : slot_out + 1;
+      const float2* here = scales_at + slot_out * T;
+      if (++slot_out == C::STAGES) { slot_out = 0; parity ^= 1u; }
       const int key0 = (s.first_chunk + c) * KEYS;
       const bool whole = key0 + KEYS <= all_to && key0 >= all_from;
       float ks[T], lv[T], iv[T];   // a page that holds nothing: log2 0 = -inf hides its keys
 #pragma unroll
       for (int h = 0; h < T; ++h) {
-        const float2 scales = *reinterpret_cast<const float2*>(here + h * C::TILE + 32 * D);
+        const float2 scales = here[h];
         const bool empty = scales.y == 0.f;
         ks[h] = empty ? 0.f : scales.x;
         lv[h] = lg2_approx(scales.y);
         iv[h] = empty ? 0.f : rcp_approx(scales.y);
       }
 
-      // ---- S^T = K . Q^T: keys g, g + 8 of a tile, rows 2t, 2t + 1.  All tiles, groups and planes step
-      // through the channels together: 2 T NG independent accumulations hide the MMA's latency ----
-      int hi[T][NG][4], lo[T][NG][4];
-#pragma unroll
-      for (int h = 0; h < T; ++h)
-#pragma unroll
-        for (int ng = 0; ng < NG; ++ng)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) hi[h][ng][e] = lo[h][ng][e] = 0;
-      uint32_t kf[T][D / 32][4];
-#pragma unroll
-      for (int w = 0; w < D / 32; ++w)
-#pragma unroll
-        for (int h = 0; h < T; ++h) ldmatrix_x4(kf[h][w], base + h * C::TILE + tile_offset<D>(m_row, 2 * w + m_piece));
-#pragma unroll
-      for (int w = 0; w < D / 32; ++w) {
-#pragma unroll
-        for (int ng = 0; ng < NG; ++ng) {
-          uint4 q4;
-          if constexpr (C::Q_REGS) q4 = qr[ng][w];
-          else q4 = my_q[(ng * (D / 32) + w) * 32];
-#pragma unroll
-          for (int h = 0; h < T; ++h) {
-            mma_s8_16832(hi[h][ng], kf[h][w], q4.x, q4.y);
-            mma_s8_16832(lo[h][ng], kf[h][w], q4.z, q4.w);
-          }
-        }
-      }
+      // ---- S^T = K . Q^T: keys g, g + 8 of a tile, rows 2t, 2t + 1.  Groups, planes (and both tiles, while the
+      // registers last) step through the channels together: four to eight independent accumulations hide the
+      // MMA's latency ----
+      constexpr int TOGETHER = NG <= 2 ? T : 1;
       float x[T][NG][4];
 #pragma unroll
-      for (int h = 0; h < T; ++h)
+      for (int h0 = 0; h0 < T; h0 += TOGETHER) {
+        int hi[TOGETHER][NG][4], lo[TOGETHER][NG][4];
 #pragma unroll
-        for (int ng = 0; ng < NG; ++ng) {
-          const float f0 = row_scale[ng][0] * ks[h], f1 = row_scale[ng][1] * ks[h];
+        for (int h = 0; h < TOGETHER; ++h)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            x[h][ng][e] = fmaf((float)(hi[h][ng][e] * 128 + lo[h][ng][e]), e & 1 ? f1 : f0, lv[h]);
+          for (int ng = 0; ng < NG; ++ng)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) hi[h][ng][e] = lo[h][ng][e] = 0;
+        uint32_t kf[TOGETHER][D / 32][4];
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w)
+#pragma unroll
+          for (int h = 0; h < TOGETHER; ++h)
+            ldmatrix_x4(kf[h][w], base + (h0 + h) * C::TILE + tile_offset<D>(m_row, 2 * w + m_piece));
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w) {
+#pragma unroll
+          for (int ng = 0; ng < NG; ++ng) {
+            uint4 q4;
+            if constexpr (C::Q_REGS) q4 = qr[ng][w];
+            else q4 = my_q[(ng * (D / 32) + w) * 32];
+#pragma unroll
+            for (int h = 0; h < TOGETHER; ++h) {
+              mma_s8_16832(hi[h][ng], kf[h][w], q4.x, q4.y);
+              mma_s8_16832(lo[h][ng], kf[h][w], q4.z, q4.w);
+            }
+          }
         }
+#pragma unroll
+        for (int h = 0; h < TOGETHER; ++h)
+#pragma unroll
+          for (int ng = 0; ng < NG; ++ng) {
+            const float f0 = row_scale[ng][0] * ks[h0 + h], f1 = row_scale[ng][1] * ks[h0 + h];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              x[h0 + h][ng][e] = fmaf((float)(hi[h][ng][e] * 128 + lo[h][ng][e]), e & 1 ? f1 : f0, lv[h0 + h]);
+          }
+      }
       if (!whole) {
 #pragma unroll
         for (int ng = 0; ng < NG; ++ng)
@@ -547,22 +569,32 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
         l += __shfl_xor_sync(0xffffffffu, l, 16);
         if (g == 0) ml[warp * NG * 8 + ng * 8 + 2 * t + e] = make_float2(m_run[ng][e], l);
       }
-    if constexpr (CLUSTER) cp_async_wait<0>();      // the ring becomes the cluster's partials
     __syncthreads();
     const bool complete = !CLUSTER && c_begin == 0 && cur.cend == s.chunks;
+    // of a cluster's block, in the ring: every chunk has been consumed
     float* const res_o = reinterpret_cast<float*>(smem);                 // [rows_per_unit][D]
     float2* const res_ml = reinterpret_cast<float2*>(res_o + a.rows_per_unit * D);
     const int64_t part = (2ll * blockIdx.x + (c_begin == 0)) * a.rows_per_unit;
-    const float2* my_ml = ml + rw * key_warps * NG * 8;
+    // per row: the weight of every key warp, and the joint reference and sum
+    for (int idx = tid; idx < a.row_warps * NG * 8; idx += kPaThreads) {
+      const int w_row = idx / (NG * 8), row = idx - w_row * NG * 8;
+      float2* mine = ml + w_row * key_warps * NG * 8 + row;
+      float m = kNegSentinel, l = 0.f;
+      for (int w = 0; w < key_warps; ++w) m = fmaxf(m, mine[w * NG * 8].x);
+      for (int w = 0; w < key_warps; ++w) {
+        const float2 one = mine[w * NG * 8];
+        const float f = ex2_approx(one.x - m);
+        l = fmaf(one.y, f, l);
+        mine[w * NG * 8].x = f;
+      }
+      joint[idx] = make_float2(m, l);
+    }
+    __syncthreads();
 #pragma unroll
     for (int ng = 0; ng < NG; ++ng) {
       float f[2];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float m = kNegSentinel;
-        for (int w = 0; w < key_warps; ++w) m = fmaxf(m, my_ml[w * NG * 8 + ng * 8 + 2 * t + e].x);
-        f[e] = ex2_approx(m_run[ng][e] - m);
-      }
+      for (int e = 0; e < 2; ++e) f[e] = ml[warp * NG * 8 + ng * 8 + 2 * t + e].x;
 #pragma unroll
       for (int d0 = 0; d0 < D; d0 += C::JOIN) {
 #pragma unroll
@@ -575,24 +607,23 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
         __syncthreads();
         for (int idx = kw * 32 + lane; idx < 2 * C::JOIN; idx += key_warps * 32) {
           const int row = idx / (C::JOIN / 4), ch = idx % (C::JOIN / 4) * 4;
-          float m = kNegSentinel, l = 0.f;
-          for (int w = 0; w < key_warps; ++w) m = fmaxf(m, my_ml[w * NG * 8 + ng * 8 + row].x);
-          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int w = 0; w < key_warps; ++w) {
-            const float2 one = my_ml[w * NG * 8 + ng * 8 + row];
-            l = fmaf(one.y, ex2_approx(one.x - m), l);
-            const float4 x = *reinterpret_cast<const float4*>(buf + ((rw * key_warps + w) * 8 + row) * C::BUF_ROW + ch);
+          const float* src = buf + (rw * key_warps * 8 + row) * C::BUF_ROW + ch;
+          float4 sum = *reinterpret_cast<const float4*>(src);
+#pragma unroll 3
+          for (int w = 1; w < key_warps; ++w) {
+            const float4 x = *reinterpret_cast<const float4*>(src + w * 8 * C::BUF_ROW);
             sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
           }
           const int r_local = (rw * NG + ng) * 8 + row, r = row0 + r_local;
+          const float2 both = joint[r_local];
           if constexpr (CLUSTER) {
             *reinterpret_cast<float4*>(res_o + r_local * D + d0 + ch) = sum;
-            if (d0 + ch == 0) res_ml[r_local] = make_float2(m, l);
+            if (d0 + ch == 0) res_ml[r_local] = both;
           } else if (complete) {
-            if (r < a.rows) store_row(a, cur.b, hkv, r, s.n, d0 + ch, sum, l);
+            if (r < a.rows) store_row(a, cur.b, hkv, r, s.n, d0 + ch, sum, both.y);
           } else {
             *reinterpret_cast<float4*>(a.part_o + (part + r_local) * D + d0 + ch) = sum;
-            if (d0 + ch == 0) *reinterpret_cast<float2*>(a.part_ml + (part + r_local) * 2) = make_float2(m, l);
+            if (d0 + ch == 0) *reinterpret_cast<float2*>(a.part_ml + (part + r_local) * 2) = both;
           }
         }
         __syncthreads();
@@ -624,7 +655,10 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const PagedA
       c_begin = 0;
     }
   }
-  cp_async_wait<0>();
+  if (!ok) {   // an expired wait: this warp's copies in flight land before its shared memory goes away
+    for (int i = 0; i < C::STAGES; ++i)
+      for (uint32_t ph = 0; ph < 2; ++ph) mbar_wait_quiet(&bars[i], ph, 10000000ull);
+  }
 }
 
 // Behind the split kernel, with its grid: block i joins the partials of the unit that begins in range i and ends
@@ -636,7 +670,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_join_kernel(const PagedAr
   const int units = a.Hkv * a.row_units;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Line line = line_of(a, units, red);
-  const unsigned per = share_of(line.total, a.blocks);
+  const unsigned per = share_of(a, line.total);
   const unsigned c0 = min(line.total, per * blockIdx.x), c1 = min(line.total, c0 + per);
   if (c0 < c1) locate(a, line, units, c1 - 1, s_last);
   __syncthreads();
@@ -709,7 +743,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_join_kernel(const PagedAr
 // Rows that one unit of the split kernel serves: 8 per group of the MMA's N axis, groups per warp (NG), warps
 // with other rows.
 struct Plan {
-  int ng, row_warps, row_units, rows_per_unit;
+  int ng, row_warps, row_units, rows_per_unit, chunk_shift;
   bool cluster;           // blocks = blocks per unit, else of the whole grid
   int blocks;
   size_t prefill_bytes;   // > 0: paged_prefill.cu serves the call, with this workspace
@@ -724,10 +758,7 @@ int page_shift_of(int page_size) {
   return -1;
 }
 
-int key_warps_of(const Plan& x) { return kPaWarps / x.row_warps; }
-
-// Chunks per warp up to which a cluster per unit is used.
-constexpr int kClusterSteps = 4;
+constexpr int kJoinSteps = 4, kClusterSteps = 8;
 
 PagedArgs args_of(const sl8_paged_cache& c, const sl8_paged_attn_params& p) {
   PagedArgs a{};
@@ -747,25 +778,31 @@ PagedArgs args_of(const sl8_paged_cache& c, const sl8_paged_attn_params& p) {
 
 Plan plan_of(const PagedArgs& a, int D) {
   Plan x{};
-  x.ng = (int)std::min<int64_t>(groups_of(D), (a.rows + 7) / 8);
+  x.prefill_bytes = a.rows >= kPrefillRows ? sl8_paged_prefill_workspace(a, D) : 0;
+  x.ng = std::min(groups_of(D), (a.rows + 7) / 8);
   x.row_warps = a.rows > 8 * groups_of(D) ? 2 : 1;   // PaCfg::ROW_WARPS
   x.rows_per_unit = x.row_warps * x.ng * 8;
   x.row_units = (a.rows + x.rows_per_unit - 1) / x.rows_per_unit;
-  const int keys = 1 << chunk_shift_of(D, x.ng);
-  const int64_t chunks = ((int64_t)a.max_tokens + keys - 1) / keys * a.B * a.Hkv * x.row_units;
-  const int64_t want = (chunks + kPaWarps - 1) / kPaWarps;
-  x.blocks = (int)(want < 1 ? 1 : (want > kNumSms ? kNumSms : want));
+  x.chunk_shift = chunk_shift_of(D, x.ng);
   // Few units of few chunks: a cluster per unit, up to eight blocks with a chunk per warp at least, as long as
-  // that is at most kClusterSteps chunks per warp and all clusters run at once (of eight blocks, sixteen do).
-  const int64_t units = (int64_t)a.B * a.Hkv * x.row_units, longest = ((int64_t)a.max_tokens + keys - 1) / keys;
+  // all clusters run at once (of eight blocks, sixteen do) and the chunks per warp are at most kJoinSteps more
+  // than the line would give: joining through global memory costs as much as that many steps (8 heads of 128,
+  // 4096 keys: 9.9 us in clusters, 14.5 on the line).  Above kClusterSteps a ragged batch would wait for its
+  // longest sequence, which the line does not.
+  const int64_t units = (int64_t)a.B * a.Hkv * x.row_units, keys = 1 << x.chunk_shift;
+  const int64_t longest = ((int64_t)a.max_tokens + keys - 1) / keys, key_warps = kPaWarps / x.row_warps;
   int per_unit = 1;
-  while (per_unit < 8 && units * per_unit * 2 <= 128 && (int64_t)per_unit * kPaWarps < longest) per_unit *= 2;
-  const int64_t steps = (longest + (int64_t)per_unit * key_warps_of(x) - 1) / ((int64_t)per_unit * key_warps_of(x));
-  if (units * per_unit <= kNumSms && steps <= kClusterSteps) {
+  while (per_unit < 8 && units * per_unit * 2 <= 128 && (int64_t)per_unit * key_warps < longest) per_unit *= 2;
+  const int64_t steps = (longest + per_unit * key_warps - 1) / (per_unit * key_warps);
+  const int64_t line_steps = (longest * units + kNumSms * key_warps - 1) / (kNumSms * key_warps);
+  if (units * per_unit <= kNumSms && steps <= kClusterSteps && steps <= line_steps + kJoinSteps) {
     x.cluster = true;
     x.blocks = per_unit;
+    return x;
   }
-  x.prefill_bytes = a.rows >= kPrefillRows ? sl8_paged_prefill_workspace(a, D) : 0;
+  const int64_t chunks = (((int64_t)a.max_tokens + (1 << x.chunk_shift) - 1) >> x.chunk_shift) * a.B * a.Hkv * x.row_units;
+  const int64_t want = (chunks + kPaWarps - 1) / kPaWarps;
+  x.blocks = (int)(want < 1 ? 1 : (want > kNumSms ? kNumSms : want));
   return x;
 }
 
@@ -793,6 +830,14 @@ int allow_smem() {
 
 template <int D, int NG>
 int launch_paged(const PagedArgs& a, bool cluster, cudaStream_t stream) {
+  using C = PaCfg<D, NG>;
+  CUtensorMap k_map{}, v_map{};   // boxes of one tile; an empty pool is never read
+  if (a.max_tokens > 0) {
+    const uint64_t page_heads = (uint64_t)a.num_pages * a.Hkv;
+    int rc = sl8_make_tmap_3d(&k_map, a.k, 1, D, 1u << a.page_shift, page_heads, C::ROW, 16, C::ROW);
+    if (rc == SL8_OK) rc = sl8_make_tmap_3d(&v_map, a.v, 1, D, 1u << a.page_shift, page_heads, C::ROW, 16, C::ROW);
+    if (rc != SL8_OK) return rc;
+  }
   const int smem = PaCfg<D, NG>::smem(a.row_warps);
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr{};
@@ -808,12 +853,12 @@ int launch_paged(const PagedArgs& a, bool cluster, cudaStream_t stream) {
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.gridDim = dim3((unsigned)(a.B * a.Hkv * a.row_units * a.blocks));
     cfg.dynamicSmemBytes = smem;
-    SL8_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_split_kernel<D, NG, true>, a));
+    SL8_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_split_kernel<D, NG, true>, k_map, v_map, a));
     return SL8_OK;
   }
   const int rc = allow_smem<D, NG, false>();
   if (rc != SL8_OK) return rc;
-  paged_split_kernel<D, NG, false><<<a.blocks, kPaThreads, smem, stream>>>(a);
+  paged_split_kernel<D, NG, false><<<a.blocks, kPaThreads, smem, stream>>>(k_map, v_map, a);
   if (cudaGetLastError() != cudaSuccess) return SL8_ERR_CUDA;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
@@ -867,8 +912,9 @@ extern "C" int sl8_attn_paged(const sl8_paged_cache* c, const sl8_paged_attn_par
   const Plan x = plan_of(a, c->D);
   uint8_t* ws = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 1023) & ~uintptr_t(1023));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  a.chunk_shift = chunk_shift_of(c->D, x.ng);
+  a.chunk_shift = x.chunk_shift;
   if (x.prefill_bytes > 0) return sl8_paged_prefill(a, c->D, ws, x.prefill_bytes, s);
+  if ((int64_t)c->num_pages * c->Hkv > 0x7fffffffll) return SL8_ERR_TOO_LARGE;
   // the line of all chunks is counted in 32 bits; its length is bounded by what can be seen
   const int64_t most = ((int64_t)a.max_tokens + 31) / 16 * p->B * c->Hkv * x.row_units;
   if ((int64_t)p->B * c->Hkv * x.row_units > 0x7fffffffll || most > 0x7fffffffll) return SL8_ERR_TOO_LARGE;
@@ -881,4 +927,12 @@ extern "C" int sl8_attn_paged(const sl8_paged_cache* c, const sl8_paged_attn_par
     case 128: return launch_paged_rows<128>(a, x.ng, x.cluster, s);
     default: return launch_paged_rows<256>(a, x.ng, x.cluster, s);
   }
+}
+
+extern "C" int sl8_paged_status(void* stream) {
+  void* word = nullptr;
+  SL8_CUDA_TRY(cudaGetSymbolAddress(&word, g_paged_wait_status));
+  const int rc = sl8_read_device_status(word, stream);
+  const int prefill = sl8_paged_prefill_status(stream);
+  return rc != SL8_OK ? rc : prefill;
 }

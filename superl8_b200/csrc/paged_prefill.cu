@@ -545,7 +545,7 @@ int sl8_paged_prefill(const PagedArgs& a, int D, void* workspace, size_t workspa
   return SL8_ERR_UNSUPPORTED;
 }
 
-extern "C" int sl8_paged_status(void* stream) {
+int sl8_paged_prefill_status(void* stream) {
   void* word = nullptr;
   SL8_CUDA_TRY(cudaGetSymbolAddress(&word, g_paged_status));
   return sl8_read_device_status(word, stream);

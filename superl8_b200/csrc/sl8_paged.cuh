@@ -1,4 +1,4 @@
-// What the two attention kernels over the paged cache share: their arguments and what a sequence asks for.
+// What the attention kernels over the paged cache share: their arguments and what a sequence asks for.
 #pragma once
 #include "sl8_common.cuh"
 
@@ -22,8 +22,8 @@ struct PagedArgs {
   int causal, window, bf16;
   int row_warps;      // warps that share a key but hold other rows (1 or 2)
   int rows_per_unit, row_units;            // rows = up to row_units * rows_per_unit
-  int blocks;         // blocks of the split kernel
-  int chunk_shift;    // log2 of the keys per warp and step
+  int blocks;         // blocks that share the line of all units (or a unit, in a cluster)
+  int chunk_shift;    // log2 of the keys of a chunk
   float scale_log2;   // softmax_scale * log2 e
 };
 
@@ -52,3 +52,4 @@ __device__ __forceinline__ Seq seq_of(const PagedArgs& a, int b) {
 // launch.  `workspace` is 1024-byte aligned.
 size_t sl8_paged_prefill_workspace(const sl8::PagedArgs& a, int D);
 int sl8_paged_prefill(const sl8::PagedArgs& a, int D, void* workspace, size_t workspace_bytes, cudaStream_t stream);
+int sl8_paged_prefill_status(void* stream);

@@ -363,6 +363,14 @@ LINE = [
     ([21000], 4, 1, 1, 128, 64, torch.float16, True, -1, None),
     ([9000, 17], 8, 1, 6, 64, 128, torch.bfloat16, True, -1, [6, 6]),
     ([9000], 2, 1, 1, 32, 256, torch.float16, True, -1, None),
+    # 9 ... 64 rows per KV head: keys on the rows of the MMA
+    ([200, 128, 129, 1, 0] * 20, 16, 2, 2, 128, 16, torch.float16, True, -1, None),
+    ([300, 77] * 40, 32, 2, 4, 64, 32, torch.bfloat16, True, 33, [4, 3] * 40),
+    ([140, 260] * 40, 10, 2, 8, 128, 64, torch.float16, True, 5, None),
+    ([90, 400, 30] * 26, 12, 2, 4, 128, 256, torch.bfloat16, False, 100, None),
+    ([3000, 2900, 2999] * 4, 12, 6, 8, 64, 128, torch.float16, True, 2500, None),
+    ([7000, 3, 0], 11, 1, 1, 128, 16, torch.float16, True, -1, None),
+    ([20, 3] * 40, 4, 2, 30, 128, 16, torch.float16, True, -1, None),   # more queries than context
 ]
 
 
