@@ -24,6 +24,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 namespace sl8 {
 namespace {
@@ -99,6 +100,13 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return y;
 }
 
+__device__ __forceinline__ void cp_async4(void* dst, const void* src, int bytes) {   // 0 bytes: zero
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -126,18 +134,21 @@ struct PaCfg {
   static constexpr int TILE = 2 * 16 * D;                                // K rows, V rows
   static constexpr int SLOT = TILES * TILE;
   static constexpr int SUBS = D <= 128 ? 1 : D / 128, ROW = D / SUBS;    // sub-tiles of at most 128 bytes a row
-  static constexpr int STAGES = D == 256 ? 2 : (D == 128 ? (TILES == 2 ? 3 : 5) : (D == 64 ? 5 : 8));
+  // What streams at the HBM's rate (one group) wants 128 KB in flight; more groups take longer per step than a
+  // load takes, and give the space to the join.
+  static constexpr int STAGES = D == 256 ? 2 : (D == 128 ? (TILES == 2 ? (NG == 1 ? 3 : 2) : 4) : (D == 64 ? 5 : 8));
   static constexpr int RING = kPaWarps * STAGES * SLOT;
   static constexpr int SIDE = kPaWarps * STAGES * (TILES * 8 + 8);       // the tiles' scales, the slots' barriers
-  static constexpr int JOIN = D >= 128 ? D / 2 : D;                      // channels joined at a time
-  static constexpr int BUF_ROW = JOIN + 8;                               // floats per row of the joining buffer
-  static constexpr int BUF = kPaWarps * 8 * BUF_ROW * 4;
+  // The join of a group of rows: every fragment (float4 a lane) of the other key warps' accumulators.  Two such
+  // buffers where several groups follow one another and the space is there.
+  static constexpr int FRAGS = D / 16, BUF_ONE = FRAGS * (kPaWarps - 1) * 512;
+  static constexpr int BUFS = NG > 1 && D < 256 ? 2 : 1, BUF = BUFS * BUF_ONE;
   static constexpr int Q_GROUP = D * 16;                                 // two int8 planes of 8 rows, fragment order
   static constexpr int ROW_WARPS = NG == groups_of(D) ? 2 : 1;           // most warps with rows of their own
   static constexpr int ML = (kPaWarps + ROW_WARPS) * NG * 8 * 8;         // per warp and row, and per row
   static constexpr bool Q_REGS = NG * D <= 256;                          // fragments of Q held in registers
   static constexpr int smem(int row_warps) { return 1024 + RING + SIDE + BUF + ML + row_warps * NG * (Q_GROUP + 32); }
-  static_assert(smem(ROW_WARPS) <= 226 * 1024, "over the shared memory of an SM");
+  static_assert(smem(ROW_WARPS) <= 227 * 1024 - 256, "over the shared memory of an SM");
 };
 
 __device__ __forceinline__ void cluster_sync() {
@@ -189,7 +200,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const __grid
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ unsigned red[kPaWarps];
   __shared__ int s_start[3];
-  float* buf = reinterpret_cast<float*>(smem + C::RING);
+  float4* buf = reinterpret_cast<float4*>(smem + C::RING);               // [fragment][other key warp][lane]
   float2* ml = reinterpret_cast<float2*>(smem + C::RING + C::BUF);       // [warp][NG * 8]
   float2* joint = ml + kPaWarps * NG * 8;                                // [row_warps * NG * 8]: reference, sum
   uint4* qf = reinterpret_cast<uint4*>(smem + C::RING + C::BUF + C::ML); // [group][D / 32][lane]
@@ -260,8 +271,59 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const __grid
   }
   open(cur, c_begin);
 
-  // Loads of a chunk: lane 16 h asks the copy engine for tile h (each tile has its own page) and carries its
-  // scales, which go to shared memory one step later.
+  // Q of a segment comes in two steps: the values (asked for early, a row per four lanes of its group's warp) and
+  // their two int8 planes in fragment order.
+  uint2 q_raw[D / 32][2];
+  auto load_q = [&](const Cursor& x) {
+    if (warp >= a.row_warps * NG) return;
+    const int head0 = x.u / a.row_units, r = (x.u - head0 * a.row_units) * a.rows_per_unit + warp * 8 + g;
+    const int i = r / a.G, head = head0 * a.G + r - i * a.G;
+    const bool live = r < a.rows && i < x.s.n;
+    const uint2* src = reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(a.q) + x.b * a.q_sb + head * a.q_sh + i * a.q_ss);
+#pragma unroll
+    for (int w = 0; w < D / 32; ++w)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) q_raw[w][h] = live ? __ldg(src + 8 * w + 4 * h + t) : make_uint2(0, 0);
+  };
+  auto split_q = [&]() {
+    if (warp >= a.row_warps * NG) return;
+    auto value = [&](uint32_t x) { return a.bf16 ? unpack2<__nv_bfloat16>(x) : unpack2<__half>(x); };
+    uint32_t bits = 0;   // the largest magnitude, compared as bits: a NaN stays the largest
+#pragma unroll
+    for (int w = 0; w < D / 32; ++w)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float2 u0 = value(q_raw[w][h].x), u1 = value(q_raw[w][h].y);
+        bits = max(bits, max(__float_as_uint(u0.x) & 0x7fffffffu, __float_as_uint(u0.y) & 0x7fffffffu));
+        bits = max(bits, max(__float_as_uint(u1.x) & 0x7fffffffu, __float_as_uint(u1.y) & 0x7fffffffu));
+      }
+    bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
+    bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 2));
+    const float top = __uint_as_float(bits);
+    const float inv = top < 1e-30f ? 0.f : 16256.f / top;   // a row of zeros has logits of zero
+#pragma unroll
+    for (int w = 0; w < D / 32; ++w) {
+      uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float2 u0 = value(q_raw[w][h].x), u1 = value(q_raw[w][h].y);
+        const float v[4] = {u0.x, u0.y, u1.x, u1.y};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int q16 = __float2int_rn(v[e] * inv);
+          const int q_hi = (q16 + 64) >> 7;
+          hi[h] |= (uint32_t)(q_hi & 255) << (8 * e);
+          lo[h] |= (uint32_t)((q16 - 128 * q_hi) & 255) << (8 * e);
+        }
+      }
+      qf[(warp * (D / 32) + w) * 32 + lane] = make_uint4(hi[0], hi[1], lo[0], lo[1]);
+    }
+    if (t == 0) qs[warp * 8 + g] = top * (1.f / 16256.f) * a.scale_log2;
+  };
+  load_q(cur);
+
+  // Loads of a chunk: lane 16 h asks the copy engine for tile h (each tile has its own page), and for its scales
+  // with two four-byte copies.
   const int l_tile = T == 2 ? lane >> 4 : 0;
   const bool loader = (lane & 15) == 0 && lane < 16 * T;
   Cursor ahead = cur;
@@ -281,37 +343,58 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const __grid
     }
     if (ahead.c < ahead.cend) find_page();
   };
-  seek();
-  float2 late = make_float2(0.f, 0.f);
-  int late_slot = -1;
-  auto issue = [&](int slot) {
-    if (late_slot >= 0 && loader) scales_at[late_slot * T + l_tile] = late;
-    late_slot = -1;
-    if (ahead.c < ahead.cend) {
-      late_slot = slot;
-      if (loader) {
-        late = make_float2(0.f, 0.f);                             // a missing page: scales of 0, nothing is seen
-        const bool held = (unsigned)page < (unsigned)a.num_pages;
-        if (held) {
-          const int ph = page * a.Hkv + a_head, row = a_tok & page_mask;
-          uint8_t* dst = ring + slot * C::SLOT + l_tile * C::TILE;
-          mbar_expect_tx(&bars[slot], C::TILE);
+  auto seek_or_find = [&]() { if (ahead.c < ahead.cend) find_page(); else seek(); };
+  // the first chunks' table entries come together: lane i of a half asks for the i-th chunk's
+  int early = -1;
+  {
+    const int c = ahead.c + (lane & 15) * key_warps, tok = (ahead.s.first_chunk + c) * KEYS + 16 * l_tile;
+    if ((lane & 15) < C::STAGES - 1 && c < ahead.cend && tok < ahead.s.len) early = __ldg(a_row + (tok >> a.page_shift));
+  }
+  auto load = [&](int slot) {   // chunk ahead.c of this segment into `slot`
+    if (loader) {
+      const bool held = (unsigned)page < (unsigned)a.num_pages;
+      const int ph = held ? page * a.Hkv + a_head : 0, row = a_tok & page_mask;
+      float2* sc = scales_at + slot * T + l_tile;                // a missing page: scales of 0, nothing is seen
+      cp_async4(&sc->x, a.ks + ph, held ? 4 : 0);
+      cp_async4(&sc->y, a.vs + ph, held ? 4 : 0);
+      if (held) {
+        uint8_t* dst = ring + slot * C::SLOT + l_tile * C::TILE;
+        mbar_expect_tx(&bars[slot], C::TILE);
 #pragma unroll
-          for (int i = 0; i < C::SUBS; ++i) {
-            tma_load_3d(dst + i * 16 * C::ROW, &k_map, &bars[slot], i * C::ROW, row, ph);
-            tma_load_3d(dst + 16 * D + i * 16 * C::ROW, &v_map, &bars[slot], i * C::ROW, row, ph);
-          }
-          late = make_float2(__ldg(a.ks + ph), __ldg(a.vs + ph));
-        } else {
-          mbar_arrive(&bars[slot]);
+        for (int i = 0; i < C::SUBS; ++i) {
+          tma_load_3d(dst + i * 16 * C::ROW, &k_map, &bars[slot], i * C::ROW, row, ph);
+          tma_load_3d(dst + 16 * D + i * 16 * C::ROW, &v_map, &bars[slot], i * C::ROW, row, ph);
         }
+      } else {
+        mbar_arrive(&bars[slot]);
       }
-      ahead.c += key_warps;
-      if (ahead.c < ahead.cend) find_page(); else seek();
     }
   };
+  auto issue = [&](int slot) {
+    if (ahead.c < ahead.cend) {
+      load(slot);
+      ahead.c += key_warps;
+      seek_or_find();
+    }
+    cp_async_commit();
+  };
+  bool first = true;            // the first chunks, as far as this segment has them
 #pragma unroll 1
-  for (int i = 0; i < C::STAGES - 1; ++i) issue(i);
+  for (int i = 0; i < C::STAGES - 1; ++i) {
+    const int entry = __shfl_sync(0xffffffffu, early, (lane & 16) + i);
+    if (first && ahead.c < ahead.cend) {
+      page = loader ? entry : -1;
+      a_tok = (ahead.s.first_chunk + ahead.c) * KEYS + 16 * l_tile;
+      load(i);
+      ahead.c += key_warps;
+      cp_async_commit();
+    } else {
+      if (first) seek();
+      first = false;
+      issue(i);
+    }
+  }
+  if (first) seek_or_find();
   int slot_in = C::STAGES - 1, slot_out = 0;
   uint32_t parity = 0;       // of slot_out's current use
   bool ok = true;            // false once a bounded wait has expired: the block runs on without waiting
@@ -325,50 +408,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const __grid
     // ================= one segment: chunks [c_begin, cur.cend) of unit (cur.b, cur.u) =================
     const int hkv = cur.u / a.row_units, row0 = (cur.u - hkv * a.row_units) * a.rows_per_unit;
     const Seq s = cur.s;
-    // ---- Q of the segment: two int8 planes in fragment order ----
-    for (int grp = warp; grp < a.row_warps * NG; grp += kPaWarps) {
-      const int r = row0 + grp * 8 + g;
-      const int i = r / a.G, head = hkv * a.G + r % a.G;
-      const bool live = r < a.rows && i < s.n;
-      const uint2* src = reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(a.q) + cur.b * a.q_sb + head * a.q_sh + i * a.q_ss);
-      uint2 raw[D / 32][2];
-#pragma unroll
-      for (int w = 0; w < D / 32; ++w)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) raw[w][h] = live ? __ldg(src + 8 * w + 4 * h + t) : make_uint2(0, 0);
-      float x[D / 32][2][4];
-      uint32_t bits = 0;   // the largest magnitude, compared as bits: a NaN stays the largest
-#pragma unroll
-      for (int w = 0; w < D / 32; ++w) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float2 u0 = a.bf16 ? unpack2<__nv_bfloat16>(raw[w][h].x) : unpack2<__half>(raw[w][h].x);
-          const float2 u1 = a.bf16 ? unpack2<__nv_bfloat16>(raw[w][h].y) : unpack2<__half>(raw[w][h].y);
-          x[w][h][0] = u0.x; x[w][h][1] = u0.y; x[w][h][2] = u1.x; x[w][h][3] = u1.y;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) bits = max(bits, __float_as_uint(x[w][h][e]) & 0x7fffffffu);
-        }
-      }
-      bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
-      bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 2));
-      const float top = __uint_as_float(bits);
-      const float inv = top < 1e-30f ? 0.f : 16256.f / top;   // a row of zeros has logits of zero
-#pragma unroll
-      for (int w = 0; w < D / 32; ++w) {
-        uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int q16 = __float2int_rn(x[w][h][e] * inv);
-            const int q_hi = (q16 + 64) >> 7;
-            hi[h] |= (uint32_t)(q_hi & 255) << (8 * e);
-            lo[h] |= (uint32_t)((q16 - 128 * q_hi) & 255) << (8 * e);
-          }
-        qf[(grp * (D / 32) + w) * 32 + lane] = make_uint4(hi[0], hi[1], lo[0], lo[1]);
-      }
-      if (t == 0) qs[grp * 8 + g] = top * (1.f / 16256.f) * a.scale_log2;
-    }
+    split_q();
     __syncthreads();
 
     // ---- the segment's rows of this warp ----
@@ -399,6 +439,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const __grid
     for (int c = cur.c; c < cur.cend; c += key_warps) {
       issue(slot_in);
       slot_in = slot_in + 1 == C::STAGES ? 0 : slot_in + 1;
+      cp_async_wait<C::STAGES - 1>();
       if (ok) ok = mbar_wait(&bars[slot_out], parity, &g_paged_wait_status);
       __syncwarp();
       const uint32_t base = ring_addr + slot_out * C::SLOT;
@@ -575,60 +616,84 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const __grid
     float* const res_o = reinterpret_cast<float*>(smem);                 // [rows_per_unit][D]
     float2* const res_ml = reinterpret_cast<float2*>(res_o + a.rows_per_unit * D);
     const int64_t part = (2ll * blockIdx.x + (c_begin == 0)) * a.rows_per_unit;
-    // per row: the weight of every key warp, and the joint reference and sum
-    for (int idx = tid; idx < a.row_warps * NG * 8; idx += kPaThreads) {
-      const int w_row = idx / (NG * 8), row = idx - w_row * NG * 8;
-      float2* mine = ml + w_row * key_warps * NG * 8 + row;
-      float m = kNegSentinel, l = 0.f;
-      for (int w = 0; w < key_warps; ++w) m = fmaxf(m, mine[w * NG * 8].x);
-      for (int w = 0; w < key_warps; ++w) {
-        const float2 one = mine[w * NG * 8];
-        const float f = ex2_approx(one.x - m);
-        l = fmaf(one.y, f, l);
-        mine[w * NG * 8].x = f;
-      }
-      joint[idx] = make_float2(m, l);
+    // per row: the weight of every key warp, and the joint reference and sum (a thread per row and key warp)
+    if (tid < a.rows_per_unit * key_warps) {
+      const int idx = tid / key_warps, w = tid - idx * key_warps, w_row = idx / (NG * 8);
+      float2* mine = ml + (w_row * key_warps + w) * NG * 8 + (idx - w_row * NG * 8);
+      const float2 one = *mine;
+      float m = one.x;
+      for (int o2 = key_warps / 2; o2; o2 >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o2));
+      const float f = ex2_approx(one.x - m);
+      float l = one.y * f;
+      for (int o2 = key_warps / 2; o2; o2 >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o2);
+      mine->x = f;
+      if (w == 0) joint[idx] = make_float2(m, l);
     }
     __syncthreads();
+    // where this thread's rows go: 2 t + e of every group
+    uint16_t* out_at[NG][2];
+    float inv[NG][2];
+    float2 both[NG][2];
 #pragma unroll
-    for (int ng = 0; ng < NG; ++ng) {
-      float f[2];
+    for (int ng = 0; ng < NG; ++ng)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) f[e] = ml[warp * NG * 8 + ng * 8 + 2 * t + e].x;
-#pragma unroll
-      for (int d0 = 0; d0 < D; d0 += C::JOIN) {
-#pragma unroll
-        for (int d = 0; d < C::JOIN / 16; ++d) {
-          float* dst = buf + (warp * 8 + 2 * t) * C::BUF_ROW + 16 * d + 2 * g;
-          const float* x = o[ng][d0 / 16 + d];
-          *reinterpret_cast<float2*>(dst) = make_float2(x[0] * f[0], x[2] * f[0]);
-          *reinterpret_cast<float2*>(dst + C::BUF_ROW) = make_float2(x[1] * f[1], x[3] * f[1]);
-        }
-        __syncthreads();
-        for (int idx = kw * 32 + lane; idx < 2 * C::JOIN; idx += key_warps * 32) {
-          const int row = idx / (C::JOIN / 4), ch = idx % (C::JOIN / 4) * 4;
-          const float* src = buf + (rw * key_warps * 8 + row) * C::BUF_ROW + ch;
-          float4 sum = *reinterpret_cast<const float4*>(src);
-#pragma unroll 3
-          for (int w = 1; w < key_warps; ++w) {
-            const float4 x = *reinterpret_cast<const float4*>(src + w * 8 * C::BUF_ROW);
-            sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
-          }
-          const int r_local = (rw * NG + ng) * 8 + row, r = row0 + r_local;
-          const float2 both = joint[r_local];
-          if constexpr (CLUSTER) {
-            *reinterpret_cast<float4*>(res_o + r_local * D + d0 + ch) = sum;
-            if (d0 + ch == 0) res_ml[r_local] = both;
-          } else if (complete) {
-            if (r < a.rows) store_row(a, cur.b, hkv, r, s.n, d0 + ch, sum, both.y);
-          } else {
-            *reinterpret_cast<float4*>(a.part_o + (part + r_local) * D + d0 + ch) = sum;
-            if (d0 + ch == 0) *reinterpret_cast<float2*>(a.part_ml + (part + r_local) * 2) = both;
-          }
-        }
-        __syncthreads();
+      for (int e = 0; e < 2; ++e) {
+        const int r_local = (rw * NG + ng) * 8 + 2 * t + e, r = row0 + r_local, i = r / a.G, head = hkv * a.G + r - i * a.G;
+        both[ng][e] = joint[r_local];
+        inv[ng][e] = (i < s.n && both[ng][e].y != 0.f) ? 1.f / both[ng][e].y : 0.f;
+        out_at[ng][e] = r < a.rows ? reinterpret_cast<uint16_t*>(a.out) + cur.b * a.o_sb + head * a.o_sh + i * a.o_ss : nullptr;
       }
-    }
+    auto put = [&](int ng, int e, int ch, float y0, float y1) {   // two channels of a row
+      const int r_local = (rw * NG + ng) * 8 + 2 * t + e;
+      if constexpr (CLUSTER) {
+        *reinterpret_cast<float2*>(res_o + r_local * D + ch) = make_float2(y0, y1);
+        if (ch == 0) res_ml[r_local] = both[ng][e];
+      } else if (complete) {
+        if (out_at[ng][e] != nullptr) {
+          const float f = inv[ng][e];
+          y0 = f == 0.f ? 0.f : y0 * f;
+          y1 = f == 0.f ? 0.f : y1 * f;
+          *reinterpret_cast<uint32_t*>(out_at[ng][e] + ch) = a.bf16 ? pack2<__nv_bfloat16>(y0, y1) : pack2<__half>(y0, y1);
+        }
+      } else {
+        *reinterpret_cast<float2*>(a.part_o + (part + r_local) * D + ch) = make_float2(y0, y1);
+        if (ch == 0) *reinterpret_cast<float2*>(a.part_ml + (part + r_local) * 2) = both[ng][e];
+      }
+    };
+    // a fragment is summed and written by one warp: d % key_warps (warps without one only hand theirs over)
+    auto join_groups = [&](auto key_warps_c) {
+      constexpr int KW = decltype(key_warps_c)::value, OWN = (C::FRAGS + KW - 1) / KW;
+#pragma unroll
+      for (int ng = 0; ng < NG; ++ng) {
+        float4* here = buf + (C::BUFS == 2 ? (ng & 1) * (C::BUF_ONE / 16) : 0) + rw * C::FRAGS * (KW - 1) * 32 + lane;
+        const float f0 = ml[warp * NG * 8 + ng * 8 + 2 * t].x, f1 = ml[warp * NG * 8 + ng * 8 + 2 * t + 1].x;
+        float4 own[OWN];
+#pragma unroll
+        for (int d = 0; d < C::FRAGS; ++d) {
+          const float4 x = make_float4(o[ng][d][0] * f0, o[ng][d][1] * f1, o[ng][d][2] * f0, o[ng][d][3] * f1);
+          if (d % KW == kw) own[d / KW] = x;
+          else here[(d * (KW - 1) + (kw < d % KW ? kw : kw - 1)) * 32] = x;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < OWN; ++k) {
+          const int d = k * KW + kw;
+          if (d < C::FRAGS) {
+            float4 x = own[k];
+#pragma unroll
+            for (int w = 0; w < KW - 1; ++w) {
+              const float4 y = here[(d * (KW - 1) + w) * 32];
+              x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) put(ng, e, 16 * d + 2 * g, e ? x.y : x.x, e ? x.w : x.z);
+          }
+        }
+        if (C::BUFS == 1 && ng + 1 < NG) __syncthreads();
+      }
+    };
+    if (C::ROW_WARPS == 2 && a.row_warps == 2) join_groups(std::integral_constant<int, kPaWarps / 2>{});
+    else join_groups(std::integral_constant<int, kPaWarps>{});
     if constexpr (CLUSTER) {
       cluster_sync();
       const int rank = blockIdx.x % a.blocks;
@@ -652,6 +717,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const __grid
     } else {
       if (cur.left <= 0) break;
       next_unit(cur);
+      load_q(cur);
       c_begin = 0;
     }
   }
