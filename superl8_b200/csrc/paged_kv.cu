@@ -41,7 +41,7 @@ struct AppendArgs {
   const int32_t* new_lens;    // nullable: M
   int B, Hq, Hkv, M, D, page_shift, max_pages, num_pages, interleaved;
   int page_slots;             // pages one sequence's new tokens can touch
-  int64_t kv_units;           // (sequence, page, head): blocks that store K, and as many that store V
+  uint32_t kv_units;          // (sequence, page, head): blocks that store K, and as many that store V
   int q_heads_per_block, q_head_groups;
 };
 
@@ -56,14 +56,20 @@ __device__ __forceinline__ void append_angles(const AppendArgs& a, const unsigne
     rope_angles<8>(a.f, table, i0, b, i, c, s);
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) rope_angle(place, table[i0 + e], c[e], s[e]);
+    for (int e = 0; e < 8; e += 2) {
+      float2 cc, ss;
+      rope_angle2(place, table[i0 + e], place, table[i0 + e + 1], cc, ss);
+      c[e] = cc.x; c[e + 1] = cc.y;
+      s[e] = ss.x; s[e + 1] = ss.y;
+    }
   }
 }
 
 __device__ __forceinline__ uint32_t pack_codes(const float* x, float inv) {
-  const uint32_t a = __float_as_uint(fmaf(x[0], inv, kMagic)), b = __float_as_uint(fmaf(x[1], inv, kMagic));
-  const uint32_t c = __float_as_uint(fmaf(x[2], inv, kMagic)), d = __float_as_uint(fmaf(x[3], inv, kMagic));
-  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+  const float2 inv2 = make_float2(inv, inv), magic2 = make_float2(kMagic, kMagic);
+  const float2 a = __ffma2_rn(make_float2(x[0], x[1]), inv2, magic2), b = __ffma2_rn(make_float2(x[2], x[3]), inv2, magic2);
+  return __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040),
+                     __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040), 0x5410);
 }
 
 __device__ __forceinline__ void store_codes(int8_t* row, int2 at, const float (&u)[8], const float (&w)[8], float inv) {
@@ -71,11 +77,20 @@ __device__ __forceinline__ void store_codes(int8_t* row, int2 at, const float (&
   *reinterpret_cast<uint2*>(row + at.y) = make_uint2(pack_codes(w, inv), pack_codes(w + 4, inv));
 }
 
+// Largest magnitude of 16 values; a NaN stays (max.NaN), unlike in fmaxf.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 __device__ __forceinline__ uint32_t abs_bits(const float (&u)[8], const float (&w)[8]) {
-  uint32_t m = 0;
+  float m = max3_abs(u[0], u[1], w[0]), k = max3_abs(w[1], u[2], w[2]);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) m = max(m, max(__float_as_uint(u[e]) & 0x7fffffffu, __float_as_uint(w[e]) & 0x7fffffffu));
-  return m;
+  for (int e = 3; e < 7; e += 2) {
+    m = max3_abs(m, u[e], u[e + 1]);
+    k = max3_abs(k, w[e], w[e + 1]);
+  }
+  return __float_as_uint(max3_abs(max3_abs(m, u[7], w[7]), k, k)) & 0x7fffffffu;
 }
 
 // Older codes of a page meet its larger scale.
@@ -98,10 +113,10 @@ __device__ __forceinline__ void requantise(int8_t* codes, int bytes, float ratio
 // NIT > 0: items (16 channels of a token) per thread, held in registers between the maximum and the
 // codes; NIT = 0: any number, read twice (the second time from L1 / L2).
 template <typename T, int NIT, bool IS_K>
-__device__ void append_page(const AppendArgs& a, int64_t unit, uint32_t* red, const unsigned long long* table) {
-  const int h = (int)(unit % a.Hkv);
-  const int64_t rest = unit / a.Hkv;
-  const int slot = (int)(rest % a.page_slots), b = (int)(rest / a.page_slots);
+__device__ void append_page(const AppendArgs& a, uint32_t unit, uint32_t* red, const unsigned long long* table) {
+  const uint32_t rest = unit / (uint32_t)a.Hkv;
+  const int h = (int)(unit - rest * a.Hkv);
+  const int b = (int)(rest / (uint32_t)a.page_slots), slot = (int)(rest - (uint32_t)b * a.page_slots);
   const int len = __ldg(a.lens + b), n = new_count(a, b);
   const int page_size = 1 << a.page_shift;
   const int64_t start = (int64_t)len - n;                          // place of new token 0 (negative: not stored)
@@ -187,14 +202,14 @@ __device__ void append_page(const AppendArgs& a, int64_t unit, uint32_t* red, co
 
 // The role of a block that rotates Q: as rope.cu, rows past new_lens are written as zeros.
 template <typename T>
-__device__ void append_query(const AppendArgs& a, int64_t block, const unsigned long long* table) {
-  const int group = (int)(block % a.q_head_groups);
-  const int per_row = a.D / 16;
-  const int64_t item = block / a.q_head_groups * blockDim.x + threadIdx.x;
-  const int64_t token = item / per_row;
-  if (token >= (int64_t)a.B * a.M) return;
-  const int j = (int)(item - token * per_row);
-  const int b = (int)(token / a.M), i = (int)(token - (int64_t)b * a.M);
+__device__ void append_query(const AppendArgs& a, uint32_t block, const unsigned long long* table) {
+  const uint32_t rest = block / (uint32_t)a.q_head_groups;
+  const int group = (int)(block - rest * a.q_head_groups);
+  const int per_row = a.D / 16, row_shift = __ffs(per_row) - 1;
+  const uint32_t item = rest * blockDim.x + threadIdx.x, token = item >> row_shift;   // the host keeps them below 2^32
+  if (token >= (uint32_t)a.B * (uint32_t)a.M) return;
+  const int j = (int)(item & (per_row - 1));
+  const int b = (int)(token / (uint32_t)a.M), i = (int)(token - (uint32_t)b * a.M);
   const int n = new_count(a, b);
   const bool real = i < n, turn = real && j * 8 < a.f.half;
   const int2 at = rope_item<8>(j, a.f.half, a.interleaved != 0);
@@ -231,7 +246,7 @@ template <typename T, int NIT>
 __global__ void __launch_bounds__(256, 3) append_kernel(const AppendArgs a) {
   __shared__ uint32_t red[8];
   __shared__ unsigned long long table[128];   // D <= 256
-  const int64_t block = blockIdx.x;
+  const uint32_t block = blockIdx.x;
   const bool v_role = block >= a.kv_units && block < 2 * a.kv_units;
   if (a.f.half > 0 && !v_role) {
     rope_table(table, a.f);
@@ -254,7 +269,7 @@ int launch_append(AppendArgs a, cudaStream_t stream) {
   const int nit = (items + threads - 1) / threads;
   a.page_slots = (a.M + page_size - 2) / page_size + 1;
   if (a.page_slots > a.max_pages) a.page_slots = a.max_pages;
-  a.kv_units = (int64_t)a.B * a.page_slots * a.Hkv;
+  const int64_t kv_units = (int64_t)a.B * a.page_slots * a.Hkv;
   int64_t q_blocks = 0;
   if (a.q) {
     // the heads of a block share the angles: at least four of them unless that leaves SMs idle
@@ -266,9 +281,10 @@ int launch_append(AppendArgs a, cudaStream_t stream) {
     a.q_head_groups = (a.Hq + a.q_heads_per_block - 1) / a.q_heads_per_block;
     q_blocks = gx * a.q_head_groups;
   }
-  const int64_t blocks = 2 * a.kv_units + q_blocks;
+  const int64_t blocks = 2 * kv_units + q_blocks;
   if (blocks == 0) return SL8_OK;
-  if (blocks > 0x7fffffffll) return SL8_ERR_TOO_LARGE;
+  if (blocks > 0x7fffffffll || (int64_t)a.B * a.M * (a.D / 16) + threads > 0xffffffffll) return SL8_ERR_TOO_LARGE;
+  a.kv_units = (uint32_t)kv_units;
   if (nit <= 1) append_kernel<T, 1><<<(unsigned)blocks, threads, 0, stream>>>(a);
   else if (nit == 2) append_kernel<T, 2><<<(unsigned)blocks, threads, 0, stream>>>(a);
   else append_kernel<T, 0><<<(unsigned)blocks, threads, 0, stream>>>(a);
@@ -284,20 +300,16 @@ struct ReadArgs {
   const int32_t* lens;
   const int32_t* first;      // nullable: 0
   int Hkv, count, D, page_shift, max_pages, num_pages;
-  int64_t rows;              // B * Hkv * count
 };
 
 // 16 codes -> 16 values; a thread's piece of a row for K and the same piece for V.
 template <typename T>
 __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
-  const int per_row = a.D / 16;
-  const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = item / per_row;
-  if (row >= a.rows) return;
-  const int j = (int)(item - row * per_row);
-  const int64_t bh = row / a.count;
-  const int i = (int)(row - bh * a.count);
-  const int b = (int)(bh / a.Hkv), h = (int)(bh - (int64_t)b * a.Hkv);
+  const int per_row = a.D / 16, row_shift = __ffs(per_row) - 1;
+  const uint32_t item = blockIdx.x * 256 + threadIdx.x;
+  const int i = (int)(item >> row_shift), j = (int)(item & (per_row - 1)), h = blockIdx.y, b = blockIdx.z;
+  if (i >= a.count) return;
+  const int64_t row = ((int64_t)b * a.Hkv + h) * a.count + i;
   const int64_t token = (a.first ? (int64_t)__ldg(a.first + b) : 0) + i;
   int page = -1;
   if (token >= 0 && token < __ldg(a.lens + b) && (token >> a.page_shift) < a.max_pages)
@@ -415,11 +427,12 @@ extern "C" int sl8_kv_read_paged(const sl8_paged_cache* c, int32_t B, const int3
     return SL8_ERR_NULL;
   }
   ReadArgs a{c->k, c->v, c->k_scale, c->v_scale, k_out, v_out, c->block_table, c->table_stride, c->context_lens, first,
-             c->Hkv, count, c->D, page_shift_of(c->page_size), held ? c->max_pages : 0, c->num_pages, rows};
-  const int64_t blocks = (rows * (c->D / 16) + 255) / 256;
-  if (blocks > 0x7fffffffll) return SL8_ERR_TOO_LARGE;
+             c->Hkv, count, c->D, page_shift_of(c->page_size), held ? c->max_pages : 0, c->num_pages};
+  const int64_t gx = ((int64_t)count * (c->D / 16) + 255) / 256;
+  if (gx * 256 > 0xffffffffll || c->Hkv > 65535 || B > 65535) return SL8_ERR_TOO_LARGE;
+  const dim3 blocks((unsigned)gx, (unsigned)c->Hkv, (unsigned)B);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == SL8_F16) read_kernel<__half><<<(unsigned)blocks, 256, 0, s>>>(a);
-  else read_kernel<__nv_bfloat16><<<(unsigned)blocks, 256, 0, s>>>(a);
+  if (dtype == SL8_F16) read_kernel<__half><<<blocks, 256, 0, s>>>(a);
+  else read_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(a);
   return cudaGetLastError() == cudaSuccess ? SL8_OK : SL8_ERR_CUDA;
 }

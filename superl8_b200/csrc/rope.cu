@@ -19,7 +19,7 @@ struct RopeTensor {
 struct RopeArgs {
   RopeTensor q, k;
   RopeFreq f;
-  int64_t tokens;   // B * S
+  uint32_t tokens;   // B * S
   int S, Hq, H, items, heads_per_block, interleaved;   // H = Hq + Hkv
 };
 
@@ -37,11 +37,11 @@ template <typename T, int VEC>
 __global__ void __launch_bounds__(kRopeThreads, RopeCfg<T, VEC>::BLOCKS) rope_kernel(const RopeArgs a) {
   constexpr int U = RopeCfg<T, VEC>::U;
   extern __shared__ unsigned long long table[];
-  const int64_t item = (int64_t)blockIdx.x * kRopeThreads + threadIdx.x;
-  const int64_t token = item / a.items;
+  const uint32_t item = blockIdx.x * kRopeThreads + threadIdx.x;   // the host keeps them below 2^32
+  const uint32_t token = item / (uint32_t)a.items;
   const bool real = token < a.tokens;
   const int j = (int)(item - token * a.items);
-  const int64_t b = token / a.S, s = token - b * a.S;
+  const int64_t b = token / (uint32_t)a.S, s = token - b * a.S;
   const bool turn = j * VEC < a.f.half;
   const bool interleaved = a.interleaved != 0;
   const int2 at = rope_item<VEC>(j, a.f.half, interleaved);
@@ -95,8 +95,8 @@ __global__ void __launch_bounds__(kRopeThreads, RopeCfg<T, VEC>::BLOCKS) rope_ke
 template <typename T, int VEC>
 int launch_rope(RopeArgs a, int D, cudaStream_t stream) {
   a.items = D / (2 * VEC);
-  const int64_t gx = (a.tokens * a.items + kRopeThreads - 1) / kRopeThreads;
-  if (gx > 0x7fffffffll) return SL8_ERR_TOO_LARGE;
+  const int64_t gx = ((int64_t)a.tokens * a.items + kRopeThreads - 1) / kRopeThreads;
+  if (gx * kRopeThreads > 0xffffffffll) return SL8_ERR_TOO_LARGE;
   // A block's heads share the angles (as much work as four heads' products): at least four of them, unless
   // that leaves SMs idle, and few enough for six waves of blocks.
   int64_t groups = (kNumSms * 18 + gx - 1) / gx, most = (a.H + 3) / 4;
@@ -154,7 +154,8 @@ extern "C" int sl8_rope(const sl8_rope_params* p, void* stream) {
   a.k = RopeTensor{p->k, p->k_out, p->k_stride_b, p->k_stride_h, p->k_stride_s, p->k_out_stride_b, p->k_out_stride_h, p->k_out_stride_s};
   a.f = RopeFreq{p->positions, p->pos_stride_axis, p->pos_stride_b, p->pos_stride_s, p->inv_freq, p->n_axes > 1 ? p->freq_axis : nullptr,
                  p->pos_is_64 != 0, p->n_axes, p->rot / 2, p->inverse ? -1.f : 1.f};
-  a.tokens = (int64_t)p->B * p->S;
+  if ((int64_t)p->B * p->S > 0xffffffffll) return SL8_ERR_TOO_LARGE;
+  a.tokens = (uint32_t)((int64_t)p->B * p->S);
   a.S = p->S; a.Hq = Hq; a.H = Hq + Hkv; a.interleaved = p->interleaved;
   const int vec = piece_size(*p, elem);
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -15,7 +15,7 @@ struct RopeFreq {
   const float* inv_freq;      // [rot / 2]
   const uint8_t* freq_axis;   // [rot / 2] or null (axis 0)
   int pos64, n_axes, half;    // half = rot / 2
-  float sin_sign;             // -1: the inverse rotation (the gradient)
+  float sin_sign;             // multiplies the sines; -1: the inverse rotation (the gradient)
 };
 
 // Angles in fixed point.  A frequency is held as its turns per position modulo one, in units of 2^-64
@@ -38,37 +38,53 @@ __device__ __forceinline__ long long rope_position(const RopeFreq& f, int axis, 
                  : (long long)__ldg(reinterpret_cast<const int*>(f.positions) + at);
 }
 
-// cos and sin of position * frequency: the quarter turn comes off the top bits, the rest is an angle in
-// [-pi/4, pi/4] and two Taylor series (the first terms left out are 2e-9 and 2.5e-8 there).
-__device__ __forceinline__ void rope_angle(long long pos, unsigned long long turns, float& c, float& s) {
-  const uint32_t u = (uint32_t)(((unsigned long long)pos * turns) >> 32) + 0x20000000u;
-  const int quarter = u >> 30;
-  const float x = (float)((int)(u & 0x3fffffffu) - 0x20000000) * (1.5707963267948966f * 0x1p-30f);
-  const float x2 = x * x;
-  float sn = fmaf(x2, 2.7557319e-6f, -1.9841270e-4f);      // 1/9!, -1/7!
-  sn = fmaf(sn, x2, 8.3333333e-3f);                         // 1/5!
-  sn = fmaf(sn, x2, -1.6666667e-1f);                        // -1/3!
-  sn = fmaf(sn * x2, x, x);
-  float cs = fmaf(x2, 2.4801587e-5f, -1.3888889e-3f);      // 1/8!, -1/6!
-  cs = fmaf(cs, x2, 4.1666667e-2f);                         // 1/4!
-  cs = fmaf(cs, x2, -0.5f);
-  cs = fmaf(cs, x2, 1.f);
-  c = quarter & 1 ? sn : cs;
-  s = quarter & 1 ? cs : sn;
-  if (quarter == 1 || quarter == 2) c = -c;
-  if (quarter >= 2) s = -s;
+// cos and sin of position * frequency for two frequencies: the quarter turn comes off the top bits, the rest is an
+// angle in [-pi/4, pi/4] and two Taylor series (the first terms left out are 2e-9 and 2.5e-8 there), on the packed
+// fp32 pipe.
+__device__ __forceinline__ void rope_angle2(long long pos0, unsigned long long turns0, long long pos1, unsigned long long turns1,
+                                            float2& c, float2& s) {
+  const uint32_t u0 = (uint32_t)(((unsigned long long)pos0 * turns0) >> 32) + 0x20000000u;
+  const uint32_t u1 = (uint32_t)(((unsigned long long)pos1 * turns1) >> 32) + 0x20000000u;
+  auto all = [](float v) { return make_float2(v, v); };
+  const float2 x = __fmul2_rn(make_float2((float)((int)(u0 & 0x3fffffffu) - 0x20000000), (float)((int)(u1 & 0x3fffffffu) - 0x20000000)),
+                              all(1.5707963267948966f * 0x1p-30f));
+  const float2 x2 = __fmul2_rn(x, x);
+  float2 sn = __ffma2_rn(x2, all(2.7557319e-6f), all(-1.9841270e-4f));      // 1/9!, -1/7!
+  sn = __ffma2_rn(sn, x2, all(8.3333333e-3f));                               // 1/5!
+  sn = __ffma2_rn(sn, x2, all(-1.6666667e-1f));                              // -1/3!
+  sn = __ffma2_rn(__fmul2_rn(sn, x2), x, x);
+  float2 cs = __ffma2_rn(x2, all(2.4801587e-5f), all(-1.3888889e-3f));      // 1/8!, -1/6!
+  cs = __ffma2_rn(cs, x2, all(4.1666667e-2f));                               // 1/4!
+  cs = __ffma2_rn(cs, x2, all(-0.5f));
+  cs = __ffma2_rn(cs, x2, all(1.f));
+  // by quarters: (cos, sin) -> (-sin, cos) -> (-cos, -sin) -> (sin, -cos)
+  auto turn = [](uint32_t u, float cv, float sv, float& co, float& so) {
+    const bool odd = (u >> 30) & 1;
+    co = __uint_as_float(__float_as_uint(odd ? sv : cv) ^ ((u + 0x40000000u) & 0x80000000u));
+    so = __uint_as_float(__float_as_uint(odd ? cv : sv) ^ (u & 0x80000000u));
+  };
+  turn(u0, cs.x, sn.x, c.x, s.x);
+  turn(u1, cs.y, sn.y, c.y, s.y);
 }
 
 // cos / sin of VEC consecutive frequencies from i0 on for the token (b, s).
 template <int VEC>
 __device__ __forceinline__ void rope_angles(const RopeFreq& f, const unsigned long long* table, int i0, int64_t b, int64_t s,
                                             float (&c)[VEC], float (&sn)[VEC]) {
-  long long pos = f.freq_axis ? 0 : rope_position(f, 0, b, s);
+  long long pos[VEC];
+  pos[0] = f.freq_axis ? 0 : rope_position(f, 0, b, s);
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    if (f.freq_axis) pos = rope_position(f, min((int)__ldg(f.freq_axis + i0 + e), f.n_axes - 1), b, s);
-    rope_angle(pos, table[i0 + e], c[e], sn[e]);
-    sn[e] *= f.sin_sign;
+  for (int e = 0; e < VEC; ++e)
+    pos[e] = f.freq_axis ? rope_position(f, min((int)__ldg(f.freq_axis + i0 + e), f.n_axes - 1), b, s) : pos[0];
+#pragma unroll
+  for (int e = 0; e < VEC; e += 2) {
+    const int e1 = VEC == 1 ? 0 : e + 1;
+    float2 cc, ss;
+    rope_angle2(pos[e], table[i0 + e], pos[e1], table[i0 + e1], cc, ss);
+    c[e] = cc.x;
+    c[e1] = VEC == 1 ? cc.x : cc.y;
+    sn[e] = ss.x * f.sin_sign;
+    sn[e1] = (VEC == 1 ? ss.x : ss.y) * f.sin_sign;
   }
 }
 
@@ -129,31 +145,34 @@ __device__ __forceinline__ Piece<T, VEC> piece_load(const T* p) {
 }
 
 // Turns the two pieces of one item.  Half layout: a[e] pairs with b[e].  Interleaved: the pieces are
-// consecutive channels and (a[0], a[1]), (a[2], a[3]) ... (b[0], b[1]) ... are the pairs.
+// consecutive channels and (a[0], a[1]), (a[2], a[3]) ... (b[0], b[1]) ... are the pairs.  Two elements per
+// instruction on the packed fp32 pipe.
 template <int VEC>
 __device__ __forceinline__ void rope_turn(float (&a)[VEC], float (&b)[VEC], const float (&c)[VEC], const float (&s)[VEC],
                                           bool interleaved) {
-  if (!interleaved) {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const float x = a[e], y = b[e];
-      a[e] = x * c[e] - y * s[e];
-      b[e] = y * c[e] + x * s[e];
-    }
-    return;
-  }
   if constexpr (VEC == 1) {
     const float x = a[0], y = b[0];
     a[0] = x * c[0] - y * s[0];
     b[0] = y * c[0] + x * s[0];
+  } else if (!interleaved) {
+#pragma unroll
+    for (int e = 0; e < VEC; e += 2) {
+      const float2 x = make_float2(a[e], a[e + 1]), y = make_float2(b[e], b[e + 1]);
+      const float2 cc = make_float2(c[e], c[e + 1]), ss = make_float2(s[e], s[e + 1]);
+      const float2 u = __ffma2_rn(x, cc, __fmul2_rn(y, make_float2(-ss.x, -ss.y))), w = __ffma2_rn(y, cc, __fmul2_rn(x, ss));
+      a[e] = u.x; a[e + 1] = u.y;
+      b[e] = w.x; b[e + 1] = w.y;
+    }
   } else {
+    auto one = [](float& x, float& y, float cv, float sv) {   // (x, y) -> (x c - y s, y c + x s)
+      const float2 r = __ffma2_rn(make_float2(x, y), make_float2(cv, cv), __fmul2_rn(make_float2(y, x), make_float2(-sv, sv)));
+      x = r.x;
+      y = r.y;
+    };
 #pragma unroll
     for (int e = 0; e < VEC / 2; ++e) {
-      const float x = a[2 * e], y = a[2 * e + 1], u = b[2 * e], w = b[2 * e + 1];
-      a[2 * e] = x * c[e] - y * s[e];
-      a[2 * e + 1] = y * c[e] + x * s[e];
-      b[2 * e] = u * c[VEC / 2 + e] - w * s[VEC / 2 + e];
-      b[2 * e + 1] = w * c[VEC / 2 + e] + u * s[VEC / 2 + e];
+      one(a[2 * e], a[2 * e + 1], c[e], s[e]);
+      one(b[2 * e], b[2 * e + 1], c[VEC / 2 + e], s[VEC / 2 + e]);
     }
   }
 }
