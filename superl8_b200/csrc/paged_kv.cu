@@ -243,7 +243,7 @@ __device__ void append_query(const AppendArgs& a, uint32_t block, const unsigned
 }
 
 template <typename T, int NIT>
-__global__ void __launch_bounds__(256, 3) append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(256, 4) append_kernel(const AppendArgs a) {
   __shared__ uint32_t red[8];
   __shared__ unsigned long long table[128];   // D <= 256
   const uint32_t block = blockIdx.x;
