@@ -104,8 +104,10 @@ int sl8_kv_read_paged(const sl8_paged_cache* cache, int32_t B, const int32_t* fi
  * place, else all of the context; window_left >= 0: only keys in (place - window_left, ...].
  * max_context_len (host): an upper bound of context_lens that sizes the launch and the workspace (keys at or
  * past it are not seen); <= 0 = max_pages * page_size.
- * Two kernels: a split one that streams the pages (rows M * Hq / Hkv up to 64: decode, drafted tokens), and a
- * tensor-memory one over a dense copy of the codes in the workspace (more rows; D 64 / 128 / 256, scale >= 0).
+ * Two kernels: a split one that streams the pages once per 64 query rows of a KV head (32 at D = 256; rows =
+ * M * Hq / Hkv: decode, drafted tokens), and a tensor-memory one over a dense copy of the codes in the workspace
+ * (D 64 / 128 / 256, scale >= 0, else SL8_ERR_UNSUPPORTED when asked for).  SL8_BACKEND_AUTO takes the split one
+ * up to 64 rows, and above whichever it estimates to be faster.
  * workspace: sl8_attn_paged_workspace() bytes, 16-byte aligned, any contents; it serves one call at a time.
  */
 typedef struct sl8_paged_attn_params {
@@ -115,6 +117,7 @@ typedef struct sl8_paged_attn_params {
   int32_t B, Hq, M;
   int32_t dtype; int32_t causal; int32_t window_left; int32_t max_context_len;
   float softmax_scale;
+  int32_t backend;        /* SL8_BACKEND_AUTO, SL8_BACKEND_MMA (split), SL8_BACKEND_TCGEN05 (tensor memory) */
 } sl8_paged_attn_params;
 size_t sl8_attn_paged_workspace(const sl8_paged_cache* cache, const sl8_paged_attn_params* p);
 int sl8_attn_paged(const sl8_paged_cache* cache, const sl8_paged_attn_params* p, void* workspace,

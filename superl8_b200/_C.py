@@ -709,14 +709,14 @@ def kv_read_paged(k_i8, k_scale, v_i8, v_scale, block_table, context_lens, num_t
 
 
 def attn_paged(q, k_i8, k_scale, v_i8, v_scale, block_table, context_lens, scale=None, causal=True, window_left=-1,
-               query_lens=None, max_context_len=0):
+               query_lens=None, max_context_len=0, backend=_lib.SL8_BACKEND_AUTO):
     """Attention of q [B, H_q, M, D] over a paged int8 cache; output like q."""
     what = "superl8_b200 attn_paged_cached"
     window_left = -1 if window_left < 0 else min(int(window_left), 0x7fffffff)
     limit = 0 if max_context_len is None else max(0, min(int(max_context_len), 0x7fffffff))
     if _compiled():
         r = _ext.attn_paged(q, k_i8, k_scale, v_i8, v_scale, block_table, context_lens, None if scale is None else float(scale),
-                            bool(causal), window_left, query_lens, limit)
+                            bool(causal), window_left, query_lens, limit, int(backend))
         _lib.launches += 2 if r.numel() else 0
         return r
     cache = _paged_cache(k_i8, k_scale, v_i8, v_scale, block_table, context_lens, what)
@@ -733,7 +733,7 @@ def attn_paged(q, k_i8, k_scale, v_i8, v_scale, block_table, context_lens, scale
         return out
     p = _lib.PagedAttnParams(q=q.data_ptr(), out=out.data_ptr(), **_steps(q, "q"), **_steps(out, "out"), query_lens=qlens, B=B,
                              Hq=Hq, M=M, dtype=_DTYPE[q.dtype], causal=int(bool(causal)), window_left=window_left,
-                             max_context_len=limit, softmax_scale=(1.0 / math.sqrt(D)) if scale is None else float(scale))
+                             max_context_len=limit, softmax_scale=(1.0 / math.sqrt(D)) if scale is None else float(scale), backend=int(backend))
     lib = _lib.load()
     with torch.cuda.device(q.device):
         nbytes = int(lib.sl8_attn_paged_workspace(C.byref(cache), C.byref(p)))

@@ -152,7 +152,7 @@ class PagedAttnParams(C.Structure):
         ("q", C.c_void_p), ("out", C.c_void_p), *[(f"{n}_stride_{d}", C.c_int64) for n in ("q", "out") for d in "bhs"],
         ("query_lens", C.c_void_p), ("B", C.c_int32), ("Hq", C.c_int32), ("M", C.c_int32),
         ("dtype", C.c_int32), ("causal", C.c_int32), ("window_left", C.c_int32), ("max_context_len", C.c_int32),
-        ("softmax_scale", C.c_float),
+        ("softmax_scale", C.c_float), ("backend", C.c_int32),
     ]
 
 

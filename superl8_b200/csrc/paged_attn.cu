@@ -815,7 +815,9 @@ struct Plan {
   size_t prefill_bytes;   // > 0: paged_prefill.cu serves the call, with this workspace
 };
 
-// Rows per (sequence, KV head) from which the tensor-memory kernel serves a call.
+// Rows per (sequence, KV head) from which the tensor-memory kernel may serve a call: up to 64 the split kernel
+// makes one pass (two at D = 256) and was slower in one of 36 measured calls only (48 rows of 16 x 8 units of
+// 1024 keys: 55 against 42 us).
 constexpr int kPrefillRows = 65;
 
 int page_shift_of(int page_size) {
@@ -842,9 +844,8 @@ PagedArgs args_of(const sl8_paged_cache& c, const sl8_paged_attn_params& p) {
   return a;
 }
 
-Plan plan_of(const PagedArgs& a, int D) {
+Plan plan_of(const PagedArgs& a, int D, int backend) {
   Plan x{};
-  x.prefill_bytes = a.rows >= kPrefillRows ? sl8_paged_prefill_workspace(a, D) : 0;
   x.ng = std::min(groups_of(D), (a.rows + 7) / 8);
   x.row_warps = a.rows > 8 * groups_of(D) ? 2 : 1;   // PaCfg::ROW_WARPS
   x.rows_per_unit = x.row_warps * x.ng * 8;
@@ -855,6 +856,18 @@ Plan plan_of(const PagedArgs& a, int D) {
   // than the line would give: joining through global memory costs as much as that many steps (8 heads of 128,
   // 4096 keys: 9.9 us in clusters, 14.5 on the line).  Above kClusterSteps a ragged batch would wait for its
   // longest sequence, which the line does not.
+  if (backend == SL8_BACKEND_TCGEN05 || (backend == SL8_BACKEND_AUTO && a.rows >= kPrefillRows)) {
+    // Every pass over the keys serves rows_per_unit rows: 0.09, 0.17 and 0.17 ns per key and KV head at D = 64, 128
+    // (64 rows) and 256 (32 rows).  The tensor-memory kernel takes the call when its estimate is lower: 128 rows of
+    // 16 x 8 units of 8192 keys 0.42 against 0.2 ms, but of 8 units of 32768 keys 0.18 against 0.43 ms, since eight
+    // row tiles leave most of the GPU idle there.
+    const double split_us = 10.0 + (double)a.B * a.Hkv * a.max_tokens * x.row_units * (D <= 64 ? 0.09e-3 : 0.17e-3);
+    const size_t bytes = sl8_paged_prefill_workspace(a, D);
+    if (bytes > 0 && (backend == SL8_BACKEND_TCGEN05 || sl8_paged_prefill_us(a, D) < split_us)) {
+      x.prefill_bytes = bytes;
+      return x;
+    }
+  }
   const int64_t units = (int64_t)a.B * a.Hkv * x.row_units, keys = 1 << x.chunk_shift;
   const int64_t longest = ((int64_t)a.max_tokens + keys - 1) / keys, key_warps = kPaWarps / x.row_warps;
   int per_unit = 1;
@@ -878,6 +891,7 @@ int paged_checks(const sl8_paged_cache* c, const sl8_paged_attn_params* p) {
   if (p->dtype != SL8_F16 && p->dtype != SL8_BF16) return SL8_ERR_BAD_DTYPE;
   if (c->num_pages < 0 || c->Hkv < 0 || c->max_pages < 0 || page_shift_of(c->page_size) < 0) return SL8_ERR_BAD_SHAPE;
   if (p->B < 0 || p->Hq < 0 || p->M < 0) return SL8_ERR_BAD_SHAPE;
+  if (p->backend != SL8_BACKEND_AUTO && p->backend != SL8_BACKEND_MMA && p->backend != SL8_BACKEND_TCGEN05) return SL8_ERR_UNSUPPORTED;
   if (p->Hq > 0 && (c->Hkv == 0 || p->Hq % c->Hkv != 0)) return SL8_ERR_BAD_SHAPE;
   return SL8_OK;
 }
@@ -954,7 +968,7 @@ using namespace sl8;
 
 extern "C" size_t sl8_attn_paged_workspace(const sl8_paged_cache* c, const sl8_paged_attn_params* p) {
   if (paged_checks(c, p) != SL8_OK || (int64_t)p->B * p->Hq * p->M == 0) return 1024;
-  const Plan x = plan_of(args_of(*c, *p), c->D);
+  const Plan x = plan_of(args_of(*c, *p), c->D, p->backend);
   if (x.prefill_bytes > 0) return 1024 + x.prefill_bytes;
   if (x.cluster) return 1024;
   return 1024 + (size_t)2 * x.blocks * x.rows_per_unit * (c->D + 2) * sizeof(float);
@@ -972,10 +986,12 @@ extern "C" int sl8_attn_paged(const sl8_paged_cache* c, const sl8_paged_attn_par
   if (p->q_stride_b % 8 || p->q_stride_h % 8 || p->q_stride_s % 8 || p->out_stride_b % 8 || p->out_stride_h % 8 || p->out_stride_s % 8)
     return SL8_ERR_MISALIGNED;
   if ((int64_t)p->M * (p->Hq / c->Hkv) > 0x7fffffffll - 128) return SL8_ERR_TOO_LARGE;
+  PagedArgs a = args_of(*c, *p);
+  const Plan x = plan_of(a, c->D, p->backend);
+  // (without a key there is nothing for the tensor-memory kernel: the split one writes the zeros)
+  if (p->backend == SL8_BACKEND_TCGEN05 && x.prefill_bytes == 0 && a.max_tokens > 0) return SL8_ERR_UNSUPPORTED;
   if (workspace == nullptr || workspace_bytes < sl8_attn_paged_workspace(c, p)) return SL8_ERR_WORKSPACE;
   if (!aligned16(workspace)) return SL8_ERR_MISALIGNED;
-  PagedArgs a = args_of(*c, *p);
-  const Plan x = plan_of(a, c->D);
   uint8_t* ws = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 1023) & ~uintptr_t(1023));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   a.chunk_shift = x.chunk_shift;

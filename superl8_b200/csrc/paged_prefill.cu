@@ -11,7 +11,8 @@
 //
 // Why a dense copy: a unit's keys are read by rows / 128 blocks (32 for 1024 tokens of 4 heads per KV head),
 // and widening in each of them would cost more issue slots than the softmax has to spare.  The copy (4 D bytes
-// per key) is made for as many units at a time as fit kGroupBytes, which also keeps it in L2.
+// per key) is made for as many units at a time as fit kGroupBytes, which keeps most of it in L2, or as fill the
+// GPU with row tiles, up to kMostBytes.
 //
 // Block = 128 query rows (token-major over the heads of one KV head) x 64-key tiles, six warps as in
 // fwd_tcgen05.cu: four softmax warps (one row per thread), a TMA producer, an MMA issuer; two blocks per SM
@@ -31,7 +32,7 @@ constexpr int kTM = 128, kTN = 64;
 constexpr int kSoftmaxWarps = 4, kProducerWarp = 4, kMmaWarp = 5;
 constexpr int kThreads = 192;
 constexpr int kScaleStages = 4;
-constexpr size_t kGroupBytes = 192u << 20;   // dense copies made at a time (one unit at least)
+constexpr size_t kGroupBytes = 192u << 20, kMostBytes = 2048u << 20;   // dense copies made at a time (one unit at least)
 
 __device__ int g_paged_status;               // zero when the library is loaded
 
@@ -472,6 +473,9 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_prefill_kern
   }
 }
 
+// Blocks that run at once.
+int slots_of(int D) { return D <= 128 ? 2 * kNumSms : kNumSms; }
+
 // Keys a dense copy is laid out for, and units copied at a time.
 struct Group {
   int n_pad;
@@ -484,9 +488,10 @@ Group group_of(const PagedArgs& a, int D) {
   g.n_pad = (int)(((int64_t)a.max_tokens + kTN - 1) / kTN * kTN);
   g.unit_bytes = (size_t)g.n_pad * D * 2;
   g.scale_bytes = (size_t)g.n_pad / 16 * sizeof(float2);
-  const int64_t all = (int64_t)a.B * a.Hkv;
-  const int64_t fit = (int64_t)(kGroupBytes / std::max<size_t>(2 * g.unit_bytes, 1));
-  g.units = std::max<int64_t>(1, std::min(std::min(all, fit), (int64_t)65535));
+  const int64_t all = (int64_t)a.B * a.Hkv, tiles = (a.rows + kTM - 1) / kTM;
+  const size_t both = std::max<size_t>(2 * g.unit_bytes, 1);
+  const int64_t wanted = std::min<int64_t>((slots_of(D) + tiles - 1) / tiles, kMostBytes / both);
+  g.units = std::max<int64_t>(1, std::min(std::min(all, std::max<int64_t>(kGroupBytes / both, wanted)), (int64_t)65535));
   return g;
 }
 
@@ -532,6 +537,17 @@ size_t sl8_paged_prefill_workspace(const PagedArgs& a, int D) {
   if (a.scale_log2 < 0.f || a.max_tokens <= 0) return 0;   // the sweep takes a group's maximum before it is scaled
   const Group g = group_of(a, D);
   return 2 * align1k(g.units * g.unit_bytes) + align1k(g.units * g.scale_bytes);
+}
+
+// Estimated time: every wave of blocks walks the longest context (0.67, 0.83 and 2.1 us per 64-key tile at
+// D = 64, 128 and 256, two blocks per SM except at 256), and the copy moves 6 D bytes per key at 6 TB/s.
+double sl8_paged_prefill_us(const PagedArgs& a, int D) {
+  const Group g = group_of(a, D);
+  const int64_t all = (int64_t)a.B * a.Hkv, tiles = (a.rows + kTM - 1) / kTM;
+  const int64_t waves = (all / g.units) * ((g.units * tiles + slots_of(D) - 1) / slots_of(D)) +
+                        (all % g.units * tiles + slots_of(D) - 1) / slots_of(D);
+  const double tile_us = D == 64 ? 0.67 : (D == 128 ? 0.83 : 2.1);
+  return 8.0 + (double)waves * g.n_pad / kTN * tile_us + (double)all * g.n_pad * 6 * D / 6e6;
 }
 
 int sl8_paged_prefill(const PagedArgs& a, int D, void* workspace, size_t workspace_bytes, cudaStream_t stream) {

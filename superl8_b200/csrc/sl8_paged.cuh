@@ -51,5 +51,6 @@ __device__ __forceinline__ Seq seq_of(const PagedArgs& a, int b) {
 // Many query rows per KV head (paged_prefill.cu): workspace it needs (0: it does not serve the call), and the
 // launch.  `workspace` is 1024-byte aligned.
 size_t sl8_paged_prefill_workspace(const sl8::PagedArgs& a, int D);
+double sl8_paged_prefill_us(const sl8::PagedArgs& a, int D);
 int sl8_paged_prefill(const sl8::PagedArgs& a, int D, void* workspace, size_t workspace_bytes, cudaStream_t stream);
 int sl8_paged_prefill_status(void* stream);

@@ -270,7 +270,7 @@ std::tuple<Tensor, Tensor> kv_read_paged(const Tensor& k_i8, const Tensor& k_sca
 
 Tensor attn_paged(const Tensor& q_in, const Tensor& k_i8, const Tensor& k_scale, const Tensor& v_i8, const Tensor& v_scale,
                   const Tensor& table, const Tensor& lens, const c10::optional<double>& scale, bool causal, int64_t window_left,
-                  const OptTensor& query_lens, int64_t max_context_len) {
+                  const OptTensor& query_lens, int64_t max_context_len, int64_t backend) {
   const at::NoGradGuard no_grad;   // the cache operators carry no gradient
   const char* what = "attn_paged_cached";
   const sl8_paged_cache c = cache_of(k_i8, k_scale, v_i8, v_scale, table, lens, what);
@@ -293,6 +293,7 @@ Tensor attn_paged(const Tensor& q_in, const Tensor& k_i8, const Tensor& k_scale,
   p.window_left = window_left < 0 ? -1 : (int)std::min<int64_t>(window_left, 0x7fffffff);
   p.max_context_len = (int)std::max<int64_t>(0, std::min<int64_t>(max_context_len, 0x7fffffff));
   p.softmax_scale = (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)c.D));
+  p.backend = (int)backend;
   const size_t bytes = sl8_attn_paged_workspace(&c, &p);
   Tensor ws = at::empty({(int64_t)bytes}, k_i8.options().dtype(at::kByte));
   check_rc(sl8_attn_paged(&c, &p, ws.data_ptr(), bytes, stream_of(k_i8)), what);
@@ -314,5 +315,5 @@ void bind_paged(pybind11::module_& m) {
         py::arg("context_lens"), py::arg("num_tokens"), py::arg("first"), py::arg("bf16"));
   m.def("attn_paged", &attn_paged, py::arg("q"), py::arg("k_i8"), py::arg("k_scale"), py::arg("v_i8"), py::arg("v_scale"),
         py::arg("block_table"), py::arg("context_lens"), py::arg("scale"), py::arg("causal"), py::arg("window_left"), py::arg("query_lens"),
-        py::arg("max_context_len"));
+        py::arg("max_context_len"), py::arg("backend"));
 }

@@ -21,7 +21,7 @@ from __future__ import annotations
 
 import torch
 
-from . import _C
+from . import _C, _lib
 
 
 def empty_paged_cache(num_pages: int, num_kv_heads: int, page_size: int, head_dim: int, device="cuda"):
@@ -63,7 +63,8 @@ def kv_read_paged(k_i8, k_scale, v_i8, v_scale, block_table, context_lens, num_t
 
 
 def attn_paged_cached(q, k_i8, k_scale, v_i8, v_scale, block_table, context_lens, *, scale: float | None = None,
-                      causal: bool = True, window_left: int = -1, query_lens=None, max_context_len: int | None = None):
+                      causal: bool = True, window_left: int = -1, query_lens=None, max_context_len: int | None = None,
+                      backend: int = _lib.SL8_BACKEND_AUTO):
     """softmax(scale q.K^T) V over the paged cache; q fp16/bf16 [B, H_q, M, D] (rotated where the cache's
     keys are), the result like q.
 
@@ -72,8 +73,9 @@ def attn_paged_cached(q, k_i8, k_scale, v_i8, v_scale, block_table, context_lens
     None: M for all; rows past it give zeros) and sees the keys up to its own place, or all of the context
     with ``causal=False``; ``window_left`` >= 0 leaves only keys in (place - window_left, ...].  A row that
     sees no key gives zeros.  ``max_context_len`` (host) is an upper bound of ``context_lens`` (keys at
-    or past it are not seen); None takes what the table can hold.  With more than 64 query rows per KV
-    head (M H_q / H_kv) the call widens the codes into a workspace of 4 D bytes per key and KV head,
-    at most 192 MiB or one (sequence, head) at a time, sized by that bound."""
+    or past it are not seen); None takes what the table can hold.  With many query rows per KV head
+    (M H_q / H_kv above 64, where it is estimated to be faster) the call runs on the tensor-memory path and
+    widens the codes into a workspace of 4 D bytes per key and KV head, at most 2 GiB or one (sequence, head)
+    at a time, sized by that bound; ``backend`` (SL8_BACKEND_MMA / SL8_BACKEND_TCGEN05) forces one of the two."""
     return _C.attn_paged(q, k_i8, k_scale, v_i8, v_scale, block_table, context_lens, scale, causal, window_left, query_lens,
-                         max_context_len)
+                         max_context_len, backend)

@@ -8,7 +8,7 @@ import torch
 
 import paged_oracle as po
 import superl8_b200 as s8
-from superl8_b200 import _C
+from superl8_b200 import _C, _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -222,7 +222,7 @@ def held_to(out, q, cache, table, lens, **kw):
     assert torch.isfinite(out.float()).all() and (off <= tol).all(), float((off / tol.clamp(min=1e-30)).max())
 
 
-def attend_case(device, case):
+def attend_case(device, case, backend=_lib.SL8_BACKEND_AUTO):
     lens, Hq, Hkv, M, D, page, dtype, causal, window, query_lens = case
     B = len(lens)
     table, pages = po.pages_for(lens, page, seed=sum(lens))
@@ -231,7 +231,7 @@ def attend_case(device, case):
     lens_t = torch.tensor(lens, dtype=torch.int32)
     ql = None if query_lens is None else torch.tensor(query_lens, dtype=torch.int32)
     out = s8.attn_paged_cached(*on(device, q, *cache, table, lens_t), causal=causal, window_left=window,
-                               query_lens=None if ql is None else ql.to(device))
+                               query_lens=None if ql is None else ql.to(device), backend=backend)
     assert out.shape == q.shape and out.dtype == dtype
     held_to(out, q, cache, table, lens, causal=causal, window=window, query_lens=query_lens)
 
@@ -340,15 +340,15 @@ def test_attend_strides_streams_and_repeats(device, binding):
     assert (one.float() - ref[:1].float()).abs().max() <= 4 * 2.0 ** -11 * ref.float().abs().max()
 
 
-@pytest.mark.parametrize("M", [1, 70])
-def test_attend_sees_no_key_past_the_stated_length(device, M):
+@pytest.mark.parametrize("M,backend", [(1, _lib.SL8_BACKEND_AUTO), (70, _lib.SL8_BACKEND_MMA), (70, _lib.SL8_BACKEND_TCGEN05)])
+def test_attend_sees_no_key_past_the_stated_length(device, M, backend):
     lens, page, D = [500, 300, 100], 64, 64
     table, pages = po.pages_for(lens, page)
     cache = po.random_cache(pages, 2, page, D)
     q = torch.randn(3, 4, M, D, generator=torch.Generator().manual_seed(9)).half()
     args = on(device, q, *cache, table, torch.tensor(lens, dtype=torch.int32))
     for limit in (500, 333, 16, 1):
-        held_to(s8.attn_paged_cached(*args, max_context_len=limit), q, cache, table, lens, limit=limit)
+        held_to(s8.attn_paged_cached(*args, max_context_len=limit, backend=backend), q, cache, table, lens, limit=limit)
 
 
 # More units than SMs, or more chunks than a cluster takes: the line of all units is cut into equal ranges
@@ -395,6 +395,9 @@ PREFILL = [  # lens, Hq, Hkv, M, D, page, dtype, causal, window, query_lens
 
 @pytest.mark.parametrize("case", PREFILL)
 def test_many_rows_against_definition(device, binding, case):
+    if case[4] != 32:
+        attend_case(device, case, _lib.SL8_BACKEND_TCGEN05)
+    attend_case(device, case, _lib.SL8_BACKEND_MMA)
     attend_case(device, case)
     assert _C.device_status() == 0
 
@@ -412,29 +415,33 @@ def test_many_rows_missing_pages_scales_and_groups(device):
     q = torch.randn(2, M, 8, 2 * D, generator=torch.Generator().manual_seed(7)).half()[..., :D].transpose(1, 2)
     lens_t = torch.tensor(lens, dtype=torch.int32)
     for scale in (None, 0.2, -0.05):
-        out = s8.attn_paged_cached(*on(device, q, *cache, table, lens_t), scale=scale)
+        out = s8.attn_paged_cached(*on(device, q, *cache, table, lens_t), scale=scale,
+                                   backend=_lib.SL8_BACKEND_AUTO if scale == -0.05 else _lib.SL8_BACKEND_TCGEN05)
         held_to(out, q, cache, table, lens, scale=scale)
+    with pytest.raises(RuntimeError, match="not supported"):
+        s8.attn_paged_cached(*on(device, q, *cache, table, lens_t), scale=-0.05, backend=_lib.SL8_BACKEND_TCGEN05)
     bad = q.clone()
     bad[1, 3, 5, 2] = float("nan")
-    out = s8.attn_paged_cached(*on(device, bad, *cache, table, lens_t))
+    out = s8.attn_paged_cached(*on(device, bad, *cache, table, lens_t), backend=_lib.SL8_BACKEND_TCGEN05)
     assert torch.isnan(out[1, 3, 5].float()).all()
     out[1, 3, 5] = 0
     assert torch.isfinite(out.float()).all()
-    # 3 x 8 units of 30016 keys at D = 128 are 369 MB of dense copies: two groups; against one sequence at a time
+    # 24 units of 200000 keys at D = 128 are 2.5 GB of dense copies: two groups; against one sequence at a time
     g = torch.Generator(device=device).manual_seed(11)
-    lens = [30000, 29000, 257]
+    lens = [200000, 29000, 257]
     table, pages = po.pages_for(lens, 128)
     big = [torch.randint(-127, 128, (pages, 8, 128, D), dtype=torch.int8, device=device, generator=g) for _ in "kv"]
     sc = [torch.rand(pages, 8, device=device, generator=g) * 0.02 + 0.01 for _ in "kv"]
     cache = (big[0], sc[0], big[1], sc[1])
     q = torch.randn(3, 16, 40, D, device=device, generator=g).half()
     args = on(device, table, torch.tensor(lens, dtype=torch.int32))
-    out = s8.attn_paged_cached(q, *cache, *args, max_context_len=30000)
+    out = s8.attn_paged_cached(q, *cache, *args, max_context_len=200000, backend=_lib.SL8_BACKEND_TCGEN05)
     for b in range(3):
-        one = s8.attn_paged_cached(q[b:b + 1], *cache, args[0][b:b + 1], args[1][b:b + 1], max_context_len=lens[b])
+        one = s8.attn_paged_cached(q[b:b + 1], *cache, args[0][b:b + 1], args[1][b:b + 1], max_context_len=lens[b],
+                                   backend=_lib.SL8_BACKEND_TCGEN05)
         assert torch.equal(out[b:b + 1], one)
     # and the first rows against the split kernel (up to 64 rows: 20 tokens of 2 heads per KV head)
-    few = s8.attn_paged_cached(q[:, :, 20:], *cache, *args, max_context_len=30000)
+    few = s8.attn_paged_cached(q[:, :, 20:], *cache, *args, max_context_len=200000)
     assert (few.float() - out[:, :, 20:].float()).abs().max() <= 0.01 * out.float().abs().max()
     assert _C.device_status() == 0
 
@@ -533,6 +540,7 @@ def test_refusals(device, binding):
         ("multiple of 16", lambda: s8.kv_append_paged(k, k, *cache, table, lens, inv_freq=inv[:3])),
         ("dtype of k", lambda: s8.kv_append_paged(k, k, *cache, table, lens, q=q.bfloat16(), inv_freq=inv)),
         ("need freq_axis", lambda: s8.kv_append_paged(k, k, *cache, table, lens, inv_freq=inv, positions=torch.zeros(2, 2, 1, dtype=torch.long, device=device))),
+        ("not supported", lambda: s8.attn_paged_cached(q, *cache, table, lens, backend=_lib.SL8_BACKEND_TCGEN05_2Q)),
         ("negative", lambda: s8.kv_read_paged(*cache, table, lens, -1)),
         ("first", lambda: s8.kv_read_paged(*cache, table, lens, 1, first=lens.long())),
         ("dtype", lambda: s8.kv_read_paged(*cache, table, lens, 1, dtype=torch.float32)),
