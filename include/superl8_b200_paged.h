@@ -23,7 +23,8 @@ extern "C" {
  * copied.  positions: int32 or int64 (pos_is_64), element strides per axis, sequence and token (0 where
  * shared); freq_axis: uint8 [rot / 2], the axis of every frequency (time / height / width; NULL = axis 0;
  * values past n_axes - 1 read the last axis).  The angle is formed in 64 bits and reduced before sin / cos,
- * so positions up to 2^31 lose nothing.  inverse != 0 turns by -t: the gradient, and the inverse.
+ * so positions up to 2^31 lose nothing; inv_freq must be
+ * finite (a frequency of NaN or infinity does not turn).  inverse != 0 turns by -t: the gradient, and the inverse.
  * dtype fp16 / bf16 / fp32 (arithmetic in fp32, one rounding); D and rot even, rot <= D; strides are in
  * elements, the channel dimension is contiguous; x and y may be the same tensor.  No counterpart on the
  * reference's attention path (its `rope` is a separate glue kernel).
@@ -71,7 +72,7 @@ typedef struct sl8_paged_cache {
  * page holds no older token;  code = rint(x / scale');  older codes become rint(code * scale / scale') when
  * the scale grew (each growth moves an older value by at most half a step).  Codes behind the sequence's
  * end are left as they were.  A NaN or infinity makes its page's scale NaN or infinite: what attends to it
- * is NaN.  A page that is written to may belong to one sequence only.  fp16 / bf16, rot % 16 == 0, rows
+ * is NaN.  A page that is written to may be named once only, by one sequence.  fp16 / bf16, rot % 16 == 0, rows
  * 16-byte aligned.
  */
 typedef struct sl8_append_params {

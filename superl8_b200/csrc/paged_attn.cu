@@ -838,8 +838,8 @@ PagedArgs args_of(const sl8_paged_cache& c, const sl8_paged_attn_params& p) {
   a.page_shift = page_shift_of(c.page_size); a.num_pages = c.num_pages;
   int64_t tokens = c.num_pages > 0 ? (int64_t)c.max_pages * c.page_size : 0;
   if (p.max_context_len > 0 && p.max_context_len < tokens) tokens = p.max_context_len;
-  a.max_tokens = (int)(tokens < 0x7fffffff ? tokens : 0x7fffffff);
-  a.causal = p.causal; a.window = p.window_left; a.bf16 = p.dtype == SL8_BF16;
+  a.max_tokens = (int)(tokens < 0x7fffff00 ? tokens : 0x7fffff00);   // tile ends stay in 32 bits
+  a.causal = p.causal; a.window = p.window_left < 0x40000000 ? p.window_left : -1; a.bf16 = p.dtype == SL8_BF16;
   a.scale_log2 = p.softmax_scale * 1.4426950408889634f;
   return a;
 }
@@ -985,7 +985,7 @@ extern "C" int sl8_attn_paged(const sl8_paged_cache* c, const sl8_paged_attn_par
   if (!aligned16(p->q) || !aligned16(p->out) || (held && (!aligned16(c->k) || !aligned16(c->v)))) return SL8_ERR_MISALIGNED;
   if (p->q_stride_b % 8 || p->q_stride_h % 8 || p->q_stride_s % 8 || p->out_stride_b % 8 || p->out_stride_h % 8 || p->out_stride_s % 8)
     return SL8_ERR_MISALIGNED;
-  if ((int64_t)p->M * (p->Hq / c->Hkv) > 0x7fffffffll - 128) return SL8_ERR_TOO_LARGE;
+  if ((int64_t)p->M * (p->Hq / c->Hkv) > 0x40000000ll) return SL8_ERR_TOO_LARGE;
   PagedArgs a = args_of(*c, *p);
   const Plan x = plan_of(a, c->D, p->backend);
   // (without a key there is nothing for the tensor-memory kernel: the split one writes the zeros)

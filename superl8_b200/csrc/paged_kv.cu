@@ -377,6 +377,7 @@ extern "C" int sl8_kv_append_paged(const sl8_paged_cache* c, const sl8_append_pa
   if (p->B < 0 || p->Hq < 0 || p->M < 0 || p->n_axes < 1) return SL8_ERR_BAD_SHAPE;
   if (p->rot < 0 || p->rot > c->D || p->rot % 16 != 0) return SL8_ERR_BAD_SHAPE;
   if (p->dtype != SL8_F16 && p->dtype != SL8_BF16) return SL8_ERR_BAD_DTYPE;
+  if (p->M > 0x40000000) return SL8_ERR_TOO_LARGE;
   if ((int64_t)p->B * p->M == 0 || c->Hkv == 0) return SL8_OK;
   if (!p->k_new || !p->v_new || (p->rot > 0 && !p->inv_freq) || (p->q && !p->q_out)) return SL8_ERR_NULL;
   // an empty pool or table stores nothing but still rotates Q

@@ -48,7 +48,7 @@ def kv_append_paged(k, v, k_i8, k_scale, v_i8, v_scale, block_table, context_len
     Per touched page and head the scale becomes max(scale of the older tokens, max|new| / 127, 2^-40), the
     new codes round(x / scale); when the scale grows, the older codes of that page are rounded again
     (each growth moves a value by at most half a step).  Whatever lies behind the last token of a page is
-    left as it was.  A page that is appended to must belong to one sequence only; places outside the table
+    left as it was.  A page that is appended to must be named once only, by one sequence; places outside the table
     and page numbers outside the cache are skipped.  A NaN or infinity makes its whole page NaN."""
     return _C.kv_append_paged(k, v, k_i8, k_scale, v_i8, v_scale, block_table, context_lens, new_lens, q, positions, inv_freq,
                               freq_axis, interleaved)

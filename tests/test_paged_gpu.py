@@ -446,6 +446,48 @@ def test_many_rows_missing_pages_scales_and_groups(device):
     assert _C.device_status() == 0
 
 
+def test_line_and_many_rows_in_graphs(device):
+    """The two kernels with a second launch behind them (partials joined, dense copies), captured and replayed over
+    new contents, two graphs side by side on two streams."""
+    g = torch.Generator(device=device).manual_seed(12)
+    lens = torch.tensor([40, 700, 333, 5] * 25, dtype=torch.int32)
+    table, pages = po.pages_for(lens, 16)
+    cache = on(device, *po.random_cache(pages, 2, 16, 64))
+    table, lens = on(device, table, lens)
+    q1 = torch.randn(100, 4, 1, 64, device=device, generator=g).half()
+    q2 = torch.randn(100, 4, 70, 64, device=device, generator=g).half()
+    calls = [lambda: s8.attn_paged_cached(q1, *cache, table, lens), lambda: s8.attn_paged_cached(q2, *cache, table, lens, max_context_len=700)]
+    eager = [c().clone() for c in calls]
+    graphs, outs = [], []
+    for c in calls:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(c())
+        graphs.append(graph)
+    lens.sub_(3)
+    want = [c().clone() for c in calls]
+    side = [torch.cuda.Stream(device) for _ in graphs]
+    for _ in range(3):
+        for s, graph in zip(side, graphs):
+            s.wait_stream(torch.cuda.current_stream(device))
+            with torch.cuda.stream(s):
+                graph.replay()
+        for s in side:
+            torch.cuda.current_stream(device).wait_stream(s)
+    assert all(torch.equal(a, b) for a, b in zip(outs, want)) and not torch.equal(outs[0], eager[0])
+    assert _C.device_status() == 0
+
+
+def test_window_of_any_size(device):
+    lens, page, D = [90, 3], 16, 64
+    table, pages = po.pages_for(lens, page)
+    cache = po.random_cache(pages, 1, page, D)
+    q = torch.randn(2, 2, 9, D, generator=torch.Generator().manual_seed(13)).half()
+    args = on(device, q, *cache, table, torch.tensor(lens, dtype=torch.int32))
+    for window in (2**31 - 1, 2**40, 2**30, 2**30 - 1):
+        held_to(s8.attn_paged_cached(*args, window_left=window), q, cache, table, lens)
+
+
 def test_serving_loop_and_graphs(device):
     """A prompt, single tokens and a piece of several tokens through append and attention, against 16-bit
     attention over the values read back; then the decode step captured twice and replayed."""

@@ -73,7 +73,7 @@ def test_rope_far_positions(device):
     """At position 2^31 - 1 a 32-bit product would be off by tens of radians."""
     g = torch.Generator().manual_seed(12)
     q = torch.randn(1, 2, 6, 64, generator=g)
-    pos = torch.tensor([0, 1, 99_999, 1_000_003, 123_456_789, 2**31 - 1])
+    pos = torch.tensor([0, -7, 99_999, 1_000_003, -123_456_789, 2**31 - 1])
     inv = freqs(64)
     y, none = s8.apply_rope(q.to(device), None, pos.to(device), inv.to(device))
     assert none is None
