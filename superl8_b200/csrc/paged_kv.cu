@@ -11,9 +11,13 @@
 //   code   = rint(x / scale'),   older codes -> rint(code * scale / scale')  when scale' > scale.
 // An append that does not raise the scale leaves the older codes alone; one that does adds at most half a
 // step of the new scale to them.  The largest |x| is compared as bits, so NaN and infinity reach the scale
-// (and from there every value of the page) instead of vanishing in a maximum.  Bound by HBM for prompts
+// (as NaN, and from there every value of the page) instead of vanishing in a maximum.  Bound by HBM for prompts
 // (2 D bytes read, D written per token, head and tensor), by launch and three dependent loads
 // (length -> page -> scale) for single tokens.
+//
+// Measured (8 KV heads of 128, 32 heads of Q rotated as well): a prompt of 4096 tokens in bf16 26.5 us (9 us
+// without Q; the rotation's instructions and the loads' latency bound it, HBM would take 10), one token of
+// each of 128 sequences 5.1 us.  Reading the prompt back as 16-bit values takes 7.7 us.
 #include "sl8_rope.cuh"
 
 namespace sl8 {
@@ -181,8 +185,10 @@ __device__ void append_page(const AppendArgs& a, uint32_t unit, uint32_t* red, c
   } else {
     __syncwarp();
   }
-  // as bits again: a NaN scale stays
+  // as bits again: a NaN scale stays, and an infinite one becomes NaN, so that no product of its codes can hide
+  // the page behind a weight of exp(-inf)
   uint32_t bits = max(__float_as_uint(old) & 0x7fffffffu, __float_as_uint(__fdiv_rn(__uint_as_float(top), 127.f)));
+  if (bits >= 0x7f800000u) bits = 0x7fffffffu;
   const float now = __uint_as_float(max(bits, __float_as_uint(kScaleFloor)));
   const float inv = 1.f / now;
   if (NIT > 0) {

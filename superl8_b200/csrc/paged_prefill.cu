@@ -18,6 +18,10 @@
 // fwd_tcgen05.cu: four softmax warps (one row per thread), a TMA producer, an MMA issuer; two blocks per SM
 // share the tensor pipe (D = 256: one).  Every wait is bounded; an expired one raises the status word that
 // sl8_paged_status reads.
+//
+// Measured (D = 128, heads 32 : 8, fp16): 1024 query tokens at the end of 9216 keys, two sequences: copy 24.5 us,
+// attention 262-269 us = 880 TFLOP/s.  The softmax warps' chain bounds it, as in the 16-bit forward, and the
+// grid is 1.73 waves of resident blocks.
 #include "sl8_paged.cuh"
 #include "sl8_softmax.cuh"
 
@@ -71,7 +75,7 @@ __global__ void __launch_bounds__(256) paged_widen_kernel(const WidenArgs w) {
       kc = *reinterpret_cast<const uint4*>(a.k + at);
       vc = *reinterpret_cast<const uint4*>(a.v + at);
       const float vs = __ldg(a.vs + ph);
-      if (vs != 0.f) {   // a page that holds nothing keeps f = 0 and lv = -inf
+      if (!(vs < kLeastScale)) {   // a page that holds nothing keeps f = 0 and lv = -inf; NaN passes
         f = __ldg(a.ks + ph) * a.scale_log2;
         lv = log2f(vs);
       }
@@ -162,7 +166,8 @@ __device__ __forceinline__ void paged_sweep(uint32_t (&r)[kTN], const float2* sc
     if (g & 1) {
       const float2 st = add2(sum_a, sum_b);
       const float lv = sc[g / 2].y;
-      sum = fmaf(st.x + st.y, lv == -INFINITY ? 0.f : ex2_approx(-lv), sum);
+      // lv = NaN: rows that see the keys have NaN weights, the others' zeros stay zeros
+      sum = fmaf(st.x + st.y, lv > -INFINITY ? ex2_approx(-lv) : 0.f, sum);
       sum_a = sum_b = make_float2(0.f, 0.f);
     }
 #pragma unroll

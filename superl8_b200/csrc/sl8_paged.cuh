@@ -4,6 +4,9 @@
 
 namespace sl8 {
 
+// A V scale below the smallest normal number marks a page that holds nothing (pages are written with 2^-40 at least).
+constexpr float kLeastScale = 1.17549435e-38f;
+
 struct PagedArgs {
   const void* q;
   int64_t q_sb, q_sh, q_ss;

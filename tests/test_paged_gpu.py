@@ -152,6 +152,26 @@ def test_append_zeros_and_what_is_not_finite(device):
         assert torch.isfinite(s8.attn_paged_cached(q, *dev, table, lens + 1).float()).all()
 
 
+def test_append_infinity_alone_in_its_page(device):
+    """What is not finite makes its page NaN whatever the signs: also as the page's only token, and read back."""
+    D, page = 64, 16
+    table = torch.tensor([[1]], dtype=torch.int32, device=device)
+    lens = torch.tensor([1], dtype=torch.int32, device=device)
+    x = torch.full((1, 1, 1, D), 0.5, device=device, dtype=torch.float16)
+    q = torch.ones(1, 2, 1, D, device=device, dtype=torch.float16)
+    q[0, 1] = -1
+    for poison in (float("inf"), -float("inf"), float("nan")):
+        bad = x.clone()
+        bad[..., 7] = poison
+        for pair in ((bad, x), (x, bad)):
+            dev = s8.empty_paged_cache(2, 1, page, D, device)
+            s8.kv_append_paged(*pair, *dev, table, lens)
+            assert torch.isnan(s8.attn_paged_cached(q, *dev, table, lens).float()).all()
+            read = s8.kv_read_paged(*dev, table, lens, 1)
+            for got, given in zip(read, pair):
+                assert torch.isnan(got.float()).all() if given is bad else torch.isfinite(got.float()).all()
+
+
 def test_append_equals_rope_then_append_and_is_repeatable(device):
     """Rotation on the way = apply_rope first (up to the 16-bit rounding between the two); twice the same bits."""
     B, Hkv, M, D, page = 3, 4, 50, 128, 32
@@ -300,6 +320,31 @@ def test_attend_ignores_what_is_not_there(device):
     none = s8.attn_paged_cached(q.to(device), *s8.empty_paged_cache(0, 2, page, D, device), torch.zeros(2, 0, dtype=torch.int32, device=device),
                                 lens_t.to(device))
     assert (none == 0).all()
+
+
+@pytest.mark.parametrize("M,backend", [(4, _lib.SL8_BACKEND_AUTO), (40, _lib.SL8_BACKEND_MMA), (40, _lib.SL8_BACKEND_TCGEN05)])
+@pytest.mark.parametrize("side", [1, 3])
+def test_attend_rows_that_do_not_see_a_bad_page(device, M, backend, side):
+    """A page whose K or V scale is NaN makes the rows that see it NaN and leaves the others alone: the last
+    page under the causal mask, an early one under a window."""
+    n, page, D, Hkv, Hq, window = 98, 16, 64, 1, 4, 34
+    table, pages = po.pages_for([n], page)
+    cache = list(po.random_cache(pages, Hkv, page, D, seed=21))
+    q = torch.randn(1, Hq, M, D, generator=torch.Generator().manual_seed(22)).half()
+    lens = torch.tensor([n], dtype=torch.int32)
+    place = torch.arange(n - M, n)
+    first_seen = (place - window + 1).clamp(min=0)
+    hits = 0
+    for at, win in ((n - 1) // page, -1), (3, window):
+        bad = [t.clone() for t in cache]
+        bad[side][int(table[0, at])] = float("nan")
+        out = s8.attn_paged_cached(*on(device, q, *bad, table, lens), window_left=win, backend=backend).cpu()
+        ref, tol = po.attend(q, *cache, table, [n], window=win)
+        sees = (place >= at * page) & ((first_seen < (at + 1) * page) if win >= 0 else torch.ones(M, dtype=torch.bool))
+        hits += int(sees.any()) * int((~sees).any())
+        assert torch.isnan(out[:, :, sees].float()).all()
+        assert ((out.double() - ref).abs() <= tol)[:, :, ~sees].all()
+    assert hits == 2
 
 
 def test_attend_long_context_offsets(device):
