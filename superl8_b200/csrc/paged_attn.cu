@@ -4,8 +4,8 @@
 // Mathematics.  s_k is constant over a page, so logit = (q . code_k) s_k, and s_v moves into the exponent:
 //   w_n = exp2(logit_n + log2 s_v(n) - M),  M = running maximum of the exponent,
 //   O = sum_n w_n code_v(n),  l = sum_n w_n / s_v(n),  out = O / l.
-// w lies in (0, 1], so its rounding to fp16 for the P.V product loses 2^-12 of each term whatever the pages'
-// scales are.  q is split into two int8 planes, q = (128 hi + lo) qs with |128 hi + lo| <= 16256 per row
+// w stays below 2^8, so its rounding to fp16 for the P.V product loses 2^-11 of each term at most whatever the
+// pages' scales are.  q is split into two int8 planes, q = (128 hi + lo) qs with |128 hi + lo| <= 16256 per row
 // (half a step is 2^-15 of the row's largest value: finer than bf16, at fp16's level for the values that
 // matter), so K's codes enter the integer MMA as they lie in memory and only V's are widened.
 //

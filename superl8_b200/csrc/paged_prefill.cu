@@ -5,8 +5,8 @@
 // scales come down to: f = s_k * softmax_scale * log2 e and lv = log2 s_v.  The second is a flash-attention
 // kernel on the tensor-memory path with
 //   x_n = (q . code_k) f_n + lv_n,   w_n = 2^(x_n - M),   O += w_n code_v(n),   l += w_n / s_v(n),
-// so neither K's nor V's scale is ever rounded into a 16-bit operand; P = w is (2^-12 of each weight in fp16,
-// 2^-9 in bf16), and the output.  f and lv are constant over 16 columns: the sweep over the logits is the
+// so neither K's nor V's scale is ever rounded into a 16-bit operand; P = w is (2^-11 of each weight: fp16 also
+// under bf16 queries, since w stays below 2^8 and V's codes are exact in either type), and the output.  f and lv are constant over 16 columns: the sweep over the logits is the
 // 16-bit forward kernel's, with one multiply-add per logit.
 //
 // Why a dense copy: a unit's keys are read by rows / 128 blocks (32 for 1024 tokens of 4 heads per KV head),
@@ -44,7 +44,8 @@ __device__ int g_paged_status;               // zero when the library is loaded
 
 struct WidenArgs {
   PagedArgs a;
-  void *k, *v;          // [units][n_pad][D]
+  void* k;              // [units][n_pad][D] of the query type
+  __half* v;            // fp16
   float2* scales;       // [units][n_pad / 16]: f, lv
   int unit0, n_pad;
 };
@@ -81,20 +82,21 @@ __global__ void __launch_bounds__(256) paged_widen_kernel(const WidenArgs w) {
       }
     }
     if (i % 16 == 0 && j == 0) w.scales[((int64_t)blockIdx.y * w.n_pad + n) / 16] = make_float2(f, lv);
-    auto put = [&](const uint4& p, void* out) {
+    auto put = [&](const uint4& p, auto* out) {
+      using T = std::remove_pointer_t<decltype(out)>;
       const uint32_t c[4] = {p.x, p.y, p.z, p.w};
       uint4 o[2];
       uint32_t* y = reinterpret_cast<uint32_t*>(o);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        y[2 * e] = pack2<VT>((float)(int8_t)c[e], (float)(int8_t)(c[e] >> 8));
-        y[2 * e + 1] = pack2<VT>((float)(int8_t)(c[e] >> 16), (float)(int8_t)(c[e] >> 24));
+        y[2 * e] = pack2<T>((float)(int8_t)c[e], (float)(int8_t)(c[e] >> 8));
+        y[2 * e + 1] = pack2<T>((float)(int8_t)(c[e] >> 16), (float)(int8_t)(c[e] >> 24));
       }
-      uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<VT*>(out) + ((int64_t)blockIdx.y * w.n_pad + n) * D + 16 * j);
+      uint4* dst = reinterpret_cast<uint4*>(out + ((int64_t)blockIdx.y * w.n_pad + n) * D + 16 * j);
       dst[0] = o[0];
       dst[1] = o[1];
     };
-    put(kc, w.k);
+    put(kc, reinterpret_cast<VT*>(w.k));
     put(vc, w.v);
   }
 }
@@ -104,7 +106,7 @@ __global__ void __launch_bounds__(256) paged_widen_kernel(const WidenArgs w) {
 // One pass over the 64 logits of this thread's row, as softmax_pass (sl8_softmax.cuh) with f and lv per 16
 // columns (sc: four float2).  FIRST && MASK leaves the finished x in r (the second pass then takes them as
 // they are); otherwise r stays as the accumulators.  mx: the largest x; sum: of w / s_v.
-template <bool MASK, bool FIRST, typename VT>
+template <bool MASK, bool FIRST>
 __device__ __forceinline__ void paged_sweep(uint32_t (&r)[kTN], const float2* sc, float neg_m, int n_block, int to, int from,
                                             uint32_t t_p, float& mx, float& sum) {
   constexpr int G = 4, NG = kTN / 2 / G;      // pairs per group, groups; two groups share a scale
@@ -171,7 +173,7 @@ __device__ __forceinline__ void paged_sweep(uint32_t (&r)[kTN], const float2* sc
       sum_a = sum_b = make_float2(0.f, 0.f);
     }
 #pragma unroll
-    for (int u = 0; u < G; ++u) pk[(g * G + u) & 15] = pack2<VT>(xc[u].x, xc[u].y);
+    for (int u = 0; u < G; ++u) pk[(g * G + u) & 15] = pack2<__half>(xc[u].x, xc[u].y);
     if (((g + 1) * G) % 16 == 0) tc_st16(t_p + 16 * (((g + 1) * G) / 16 - 1), pk);
   }
   if (FIRST && MASK) mx = fmaxf(mx0, mx1);
@@ -317,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_prefill_kern
     // ======================= issuer: QK_0, QK_1, then P.V_j, QK_{j+2} =======================
     constexpr uint32_t fmt = std::is_same<VT, __nv_bfloat16>::value ? 1u : 0u;
     const uint32_t idesc_qk = umma_idesc(1, fmt, fmt, 0, 0, kTM, kTN);
-    const uint32_t idesc_pv = umma_idesc(1, fmt, fmt, 0, 1, kTM, D);
+    const uint32_t idesc_pv = umma_idesc(1, 0, 0, 0, 1, kTM, D);   // P and V are fp16
     const uint64_t dq = umma_smem_desc(smem_u32(smem + C::OFF_Q), 16, 1024, kUmmaSw128);
     const uint64_t dk = umma_smem_desc(smem_u32(smem + C::OFF_K), 16, 1024, kUmmaSw128);
     const uint64_t dv = umma_smem_desc(smem_u32(smem + C::OFF_V), C::KV_SUB, 1024, kUmmaSw128);
@@ -394,8 +396,8 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_prefill_kern
       const bool masked = n_block + kTN > all_to || n_block < all_from;
       float mx, psum;
       const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
-      if (masked) paged_sweep<true, true, VT>(acc, sc, neg_m, n_block, to, from, t_s, mx, psum);
-      else paged_sweep<false, true, VT>(acc, sc, neg_m, n_block, to, from, t_s, mx, psum);
+      if (masked) paged_sweep<true, true>(acc, sc, neg_m, n_block, to, from, t_s, mx, psum);
+      else paged_sweep<false, true>(acc, sc, neg_m, n_block, to, from, t_s, mx, psum);
       const bool grow = m_run == -INFINITY ? mx > -INFINITY : mx > m_run + kLazyRescaleLog2;
       float resc = 1.f;
       if (__any_sync(0xffffffffu, grow)) {
@@ -425,8 +427,8 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_prefill_kern
         tc_wait_st();   // the speculative P is done before P is stored again
         float unused;
         const float again = m_run == -INFINITY ? 0.f : -m_run;
-        if (masked) paged_sweep<true, false, VT>(acc, sc, again, n_block, to, from, t_s, unused, psum);
-        else paged_sweep<false, false, VT>(acc, sc, again, n_block, to, from, t_s, unused, psum);
+        if (masked) paged_sweep<true, false>(acc, sc, again, n_block, to, from, t_s, unused, psum);
+        else paged_sweep<false, false>(acc, sc, again, n_block, to, from, t_s, unused, psum);
       }
       l_run = l_run * resc + psum;
       loaded = false;
@@ -523,7 +525,7 @@ int launch_prefill(const PagedArgs& a, uint8_t* ws, cudaStream_t stream) {
   const int64_t all = (int64_t)a.B * a.Hkv;
   for (int64_t u0 = 0; u0 < all; u0 += g.units) {
     const unsigned units = (unsigned)std::min(g.units, all - u0);
-    const WidenArgs wa{a, k, v, scales, (int)u0, g.n_pad};
+    const WidenArgs wa{a, k, reinterpret_cast<__half*>(v), scales, (int)u0, g.n_pad};
     paged_widen_kernel<D, VT><<<dim3(g.n_pad / kTN, units), 256, 0, stream>>>(wa);
     const PrefillArgs pa{a, scales, (int)u0, g.n_pad};
     paged_prefill_kernel<D, VT><<<dim3((a.rows + kTM - 1) / kTM, units), kThreads, C::SMEM, stream>>>(k_map, v_map, pa);

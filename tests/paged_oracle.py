@@ -67,15 +67,14 @@ def dequant(codes, scale, table, n, first=0):
 def attend(q, k_i8, k_scale, v_i8, v_scale, table, lens, scale=None, causal=True, window=-1, query_lens=None,
            limit=None):
     """(out, tolerance) fp64 [B, Hq, M, D]; the tolerance bounds a kernel that splits q into two int8 planes (or
-    takes it as it is), rounds the weights to q's 16-bit type (or fp16) against their maximum, sums in fp32 and
+    takes it as it is), rounds the weights to fp16 against their maximum, sums in fp32 and
     rounds once at the end.  Keys at or past ``limit`` are not seen."""
     q_dt = q.dtype
     B, Hq, M, D = q.shape
     P, H, page, _ = k_i8.shape
     G = Hq // H
     scale = D ** -0.5 if scale is None else scale
-    # up to 64 rows per KV head the weights are fp16, above (the tensor-memory kernel) they have q's type
-    weight_err = U[q_dt] if M * G > 64 else U[torch.float16]
+    weight_err = U[torch.float16]
     out, tol = torch.zeros(B, Hq, M, D, dtype=F64), torch.zeros(B, Hq, M, D, dtype=F64)
     for b in range(B):
         row = table[b].tolist()
