@@ -535,7 +535,7 @@ def attn_bwd(q, k, v, o, do_, lse, scale, causal=False, *, backend=_lib.SL8_BACK
 
 def _rows(t, aligned):
     """``t`` itself when the kernels can take its rows in place, else a contiguous copy."""
-    ok = t.stride(3) == 1 or t.shape[3] == 1
+    ok = (t.stride(3) == 1 or t.shape[3] == 1) and all(t.shape[d] <= 1 or t.stride(d) != 1 for d in range(3))
     if aligned and ok:
         ok = t.data_ptr() % 16 == 0 and all(t.shape[d] <= 1 or t.stride(d) % 8 == 0 for d in range(3))
     return t if ok else t.detach().clone(memory_format=torch.contiguous_format)

@@ -38,9 +38,11 @@ void check_on(const Tensor& t, const Tensor& like, const char* what) {
 }
 
 // Rows the kernels can take in place: contiguous channels (and, for the 16-byte loads of the cache kernels,
-// aligned rows); anything else is copied.
+// aligned rows); anything else is copied.  So are rows that overlap with a step of one element: a result laid out
+// like them would not have contiguous channels.
 Tensor rows(const Tensor& t, bool aligned) {
   bool ok = t.stride(3) == 1 || t.size(3) == 1;
+  for (int d = 0; d < 3; ++d) ok = ok && (t.size(d) <= 1 || t.stride(d) != 1);
   if (aligned && ok) {
     ok = reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
     for (int d = 0; d < 3; ++d) ok = ok && (t.size(d) <= 1 || t.stride(d) % 8 == 0);

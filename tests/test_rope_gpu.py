@@ -101,6 +101,18 @@ def test_rope_strides_and_empty(device):
         assert y.shape == shape
 
 
+@pytest.mark.parametrize("S,D", [(16, 32), (40, 32)])
+def test_rope_of_overlapping_rows(device, S, D):
+    """Rows one element apart, and heads that are one tensor seen several times."""
+    flat = torch.randn(200, generator=torch.Generator().manual_seed(5)).half()
+    pos, inv = torch.arange(S), freqs(D)
+    for strides in ((0, 0, 1, 1), (0, 1, 0, 1), (0, 0, 2, 1), (0, 0, 0, 1)):
+        q = flat.as_strided((1, 3, S, D), strides)
+        y, none = s8.apply_rope(flat.to(device).as_strided((1, 3, S, D), strides), None, pos.to(device), inv.to(device))
+        assert none is None
+        held_to(y, q, torch.float16, pos, inv)
+
+
 def test_rope_gradient_against_the_formula_and_differences(device):
     g = torch.Generator().manual_seed(14)
     pos, inv = torch.randint(0, 300, (3, 2, 21), generator=g), freqs(48)
