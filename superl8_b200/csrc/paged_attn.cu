@@ -89,10 +89,14 @@ __device__ __forceinline__ void locate(const PagedArgs& a, const Line& line, int
   }
 }
 
-// Chunks per block: equal shares, whole rounds of the block's warps.
-__device__ __forceinline__ unsigned share_of(const PagedArgs& a, unsigned total) {
+// Chunks per block: equal shares, in whole rounds of the block's warps, or, where the units are shorter than that
+// on average, in whole units of the average's next power of two (256 units of 16 keys: one or two units per block
+// instead of eight on a few blocks).
+__device__ __forceinline__ unsigned share_of(const PagedArgs& a, int units, unsigned total) {
   const unsigned per = (total + a.blocks - 1) / a.blocks;
-  return max((unsigned)kPaWarps, (per + kPaWarps - 1) / kPaWarps * kPaWarps);
+  unsigned round = 1;
+  while (round < (unsigned)kPaWarps && (uint64_t)round * units * a.B < total) round *= 2;
+  return max(round, (per + round - 1) / round * round);
 }
 
 __device__ __forceinline__ float lg2_approx(float x) {
@@ -264,7 +268,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_split_kernel(const __grid
     cur.left = min(per, cur.s.chunks - c_begin);
   } else {
     const Line line = line_of(a, units, red);
-    const unsigned per = share_of(a, line.total);
+    const unsigned per = share_of(a, units, line.total);
     const unsigned c0 = min(line.total, per * blockIdx.x);
     const unsigned c1 = min(line.total, c0 + per);
     if (c0 >= c1) return;
@@ -744,7 +748,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_join_kernel(const PagedAr
   const int units = a.Hkv * a.row_units;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Line line = line_of(a, units, red);
-  const unsigned per = share_of(a, line.total);
+  const unsigned per = share_of(a, units, line.total);
   const unsigned c0 = min(line.total, per * blockIdx.x), c1 = min(line.total, c0 + per);
   if (c0 < c1) locate(a, line, units, c1 - 1, s_last);
   __syncthreads();
@@ -888,8 +892,7 @@ Plan plan_of(const PagedArgs& a, int D, int backend) {
     return x;
   }
   const int64_t chunks = (((int64_t)a.max_tokens + (1 << x.chunk_shift) - 1) >> x.chunk_shift) * a.B * a.Hkv * x.row_units;
-  const int64_t want = (chunks + kPaWarps - 1) / kPaWarps;
-  x.blocks = (int)(want < 1 ? 1 : (want > kNumSms ? kNumSms : want));
+  x.blocks = (int)(chunks < 1 ? 1 : (chunks > kNumSms ? kNumSms : chunks));
   return x;
 }
 

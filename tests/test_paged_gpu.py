@@ -491,6 +491,24 @@ def test_many_rows_missing_pages_scales_and_groups(device):
     assert _C.device_status() == 0
 
 
+@pytest.mark.parametrize("M,Hq,D", [(1, 16, 128), (3, 8, 64), (2, 16, 256), (9, 8, 32)])
+@pytest.mark.parametrize("longest", [3, 40, 200])
+def test_many_short_contexts(device, M, Hq, D, longest):
+    """More (sequence, head) units than blocks, a chunk or less each, some empty, one far longer: the bound given and not."""
+    B, Hkv, page = 90, 2, 16
+    g = torch.Generator().manual_seed(longest + M)
+    lens = torch.randint(0, longest + 1, (B,), generator=g).tolist()
+    lens[37] = 3 * longest + 160
+    table, pages = po.pages_for(lens, page, seed=longest)
+    cache = po.random_cache(pages, Hkv, page, D, seed=M)
+    q = torch.randn(B, Hq, M, D, generator=g).half()
+    dev = on(device, q, *cache, table, torch.tensor(lens, dtype=torch.int32))
+    out = s8.attn_paged_cached(*dev, max_context_len=max(lens))
+    held_to(out, q, cache, table, lens)
+    held_to(s8.attn_paged_cached(*dev), q, cache, table, lens)
+    assert torch.equal(out, s8.attn_paged_cached(*dev, max_context_len=max(lens)))
+
+
 def test_line_and_many_rows_in_graphs(device):
     """The two kernels with a second launch behind them (partials joined, dense copies), captured and replayed over
     new contents, two graphs side by side on two streams."""
