@@ -827,10 +827,9 @@ struct Plan {
   size_t prefill_bytes;   // > 0: paged_prefill.cu serves the call, with this workspace
 };
 
-// Rows per (sequence, KV head) from which the tensor-memory kernel may serve a call: up to 64 the split kernel
-// makes one pass (two at D = 256) and was slower in one of 36 measured calls only (48 rows of 16 x 8 units of
-// 1024 keys: 55 against 42 us).
-constexpr int kPrefillRows = 65;
+// Rows per (sequence, KV head) from which the tensor-memory kernel may serve a call: up to 32 the split kernel makes
+// one pass with half the work per key that its estimate below counts.
+constexpr int kPrefillRows = 33;
 
 int page_shift_of(int page_size) {
   for (int s = 4; s <= 8; ++s)
@@ -864,29 +863,35 @@ Plan plan_of(const PagedArgs& a, int D, int backend) {
   x.row_units = (a.rows + x.rows_per_unit - 1) / x.rows_per_unit;
   x.chunk_shift = chunk_shift_of(D, x.ng);
   // Few units of few chunks: a cluster per unit, up to eight blocks with a chunk per warp at least, as long as
-  // all clusters run at once (of eight blocks, sixteen do) and the chunks per warp are at most kJoinSteps more
-  // than the line would give: joining through global memory costs as much as that many steps (8 heads of 128,
-  // 4096 keys: 9.9 us in clusters, 14.5 on the line).  Above kClusterSteps a ragged batch would wait for its
-  // longest sequence, which the line does not.
+  // all clusters run at once (of eight blocks, fifteen or sixteen do, depending on which SMs a GPU has, and one too
+  // many doubles the time: 16 units of 4096 keys 18 us, 12 in clusters of four; so fourteen) and the chunks per warp
+  // are at most kJoinSteps more than the line would give: joining through global memory costs as much as that many
+  // steps (8 heads of 128, 4096 keys: 9.9 us in clusters, 14.5 on the line).  Above kClusterSteps a ragged batch
+  // would wait for its longest sequence, which the line does not.
+  const int64_t units = (int64_t)a.B * a.Hkv * x.row_units, keys = 1 << x.chunk_shift;
+  const int64_t longest = ((int64_t)a.max_tokens + keys - 1) / keys, key_warps = kPaWarps / x.row_warps;
+  int per_unit = 1;
+  while (per_unit < 8 && units * per_unit * 2 <= (per_unit == 4 ? 112 : 128) && (int64_t)per_unit * key_warps < longest) per_unit *= 2;
+  const int64_t steps = (longest + per_unit * key_warps - 1) / (per_unit * key_warps);
+  const int64_t line_steps = (longest * units + kNumSms * key_warps - 1) / (kNumSms * key_warps);
+  const bool cluster = units * per_unit <= kNumSms && steps <= kClusterSteps && steps <= line_steps + kJoinSteps;
   if (backend == SL8_BACKEND_TCGEN05 || (backend == SL8_BACKEND_AUTO && a.rows >= kPrefillRows)) {
-    // Every pass over the keys serves rows_per_unit rows: 0.09, 0.17 and 0.17 ns per key and KV head at D = 64, 128
-    // (64 rows) and 256 (32 rows).  The tensor-memory kernel takes the call when its estimate is lower: 128 rows of
-    // 16 x 8 units of 8192 keys 0.42 against 0.2 ms, but of 8 units of 32768 keys 0.18 against 0.43 ms, since eight
-    // row tiles leave most of the GPU idle there.
-    const double split_us = 10.0 + (double)a.B * a.Hkv * a.max_tokens * x.row_units * (D <= 64 ? 0.09e-3 : 0.17e-3);
+    // The tensor-memory kernel takes the call when its estimate is lower.  The split kernel's: 0.09, 0.17 and 0.17 ns
+    // per key, KV head and pass at D = 64, 128 (64 rows a pass) and 256 (32), and 6.7, 9.5 and 8.8 us per unit that a
+    // block begins, joins or leaves.  Over 439 calls (40 ... 1024 rows, 8 ... 512 units, 16 ... 16384 keys) the choice
+    // costs 0.2 % over the faster kernel's time on average and 20 % at most (64 rows of 512 units of 4096 keys: 414
+    // against 492 us); the two differ by up to three times either way (64 rows of 8 units of 16384 keys: 71 against
+    // 197 us, 72 rows of 512 units of 16 keys: 81 against 24 us).
+    const double unit_us = D <= 64 ? 6.7 : (D == 128 ? 9.5 : 8.8), begun = std::max(1.0, (double)units / kNumSms);
+    const double split_us = 4.0 + (cluster ? 1.0 : begun + 1.5) * unit_us +
+                            (double)units * a.max_tokens * (D <= 64 ? 0.09e-3 : 0.17e-3);
     const size_t bytes = sl8_paged_prefill_workspace(a, D);
     if (bytes > 0 && (backend == SL8_BACKEND_TCGEN05 || sl8_paged_prefill_us(a, D) < split_us)) {
       x.prefill_bytes = bytes;
       return x;
     }
   }
-  const int64_t units = (int64_t)a.B * a.Hkv * x.row_units, keys = 1 << x.chunk_shift;
-  const int64_t longest = ((int64_t)a.max_tokens + keys - 1) / keys, key_warps = kPaWarps / x.row_warps;
-  int per_unit = 1;
-  while (per_unit < 8 && units * per_unit * 2 <= 128 && (int64_t)per_unit * key_warps < longest) per_unit *= 2;
-  const int64_t steps = (longest + per_unit * key_warps - 1) / (per_unit * key_warps);
-  const int64_t line_steps = (longest * units + kNumSms * key_warps - 1) / (kNumSms * key_warps);
-  if (units * per_unit <= kNumSms && steps <= kClusterSteps && steps <= line_steps + kJoinSteps) {
+  if (cluster) {
     x.cluster = true;
     x.blocks = per_unit;
     return x;

@@ -547,14 +547,16 @@ size_t sl8_paged_prefill_workspace(const PagedArgs& a, int D) {
 }
 
 // Estimated time: every wave of blocks walks the longest context (0.67, 0.83 and 1.2 us per 64-key tile at
-// D = 64, 128 and 256, two blocks per SM except at 256), and the copy moves 6 D bytes per key at 6 TB/s.
+// D = 64, 128 and 256, two blocks per SM except at 256) behind 4 us of set-up, and the copy moves 6 D bytes per key,
+// Q and the result 4 D per row, at 6 TB/s.
 double sl8_paged_prefill_us(const PagedArgs& a, int D) {
   const Group g = group_of(a, D);
   const int64_t all = (int64_t)a.B * a.Hkv, tiles = (a.rows + kTM - 1) / kTM;
   const int64_t waves = (all / g.units) * ((g.units * tiles + slots_of(D) - 1) / slots_of(D)) +
                         (all % g.units * tiles + slots_of(D) - 1) / slots_of(D);
   const double tile_us = D == 64 ? 0.67 : (D == 128 ? 0.83 : 1.2);
-  return 8.0 + (double)waves * g.n_pad / kTN * tile_us + (double)all * g.n_pad * 6 * D / 6e6;
+  return (D == 256 ? 9.0 : 5.0) + (double)waves * ((double)g.n_pad / kTN * tile_us + 4.0) + (double)all * g.n_pad * 6 * D / 6e6 +
+         (double)all * a.rows * 4 * D / 6e6;
 }
 
 int sl8_paged_prefill(const PagedArgs& a, int D, void* workspace, size_t workspace_bytes, cudaStream_t stream) {

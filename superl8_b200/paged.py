@@ -74,7 +74,7 @@ def attn_paged_cached(q, k_i8, k_scale, v_i8, v_scale, block_table, context_lens
     with ``causal=False``; ``window_left`` >= 0 leaves only keys in (place - window_left, ...].  A row that
     sees no key gives zeros.  ``max_context_len`` (host) is an upper bound of ``context_lens`` (keys at
     or past it are not seen); None takes what the table can hold.  With many query rows per KV head
-    (M H_q / H_kv above 64, where it is estimated to be faster) the call runs on the tensor-memory path and
+    (M H_q / H_kv above 32, where it is estimated to be faster) the call runs on the tensor-memory path and
     widens the codes into a workspace of 4 D bytes per key and KV head, at most 2 GiB or one (sequence, head)
     at a time, sized by that bound; ``backend`` (SL8_BACKEND_MMA / SL8_BACKEND_TCGEN05) forces one of the two."""
     return _C.attn_paged(q, k_i8, k_scale, v_i8, v_scale, block_table, context_lens, scale, causal, window_left, query_lens,
